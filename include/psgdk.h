@@ -29,7 +29,8 @@
 extern "C" {
 #endif
 
-#define PSGDK_VERSION 404    /* round 6 (404): psgdk_lra_info (which row kernels the last LRA call took);
+#define PSGDK_VERSION 405    /* 405: microscaled (MX) numbers (psgdk_mx_*, psgdk_rms_norm_mx*), PSGDK_F16;
+                                round 6 (404): psgdk_lra_info (which row kernels the last LRA call took);
                                 round 6 (403): psgdk_flat_set_clip_groups / psgdk_flat_apply_groups, psgdk_export_precond_grad clip = 2 (deferred clip of row shards),
                                 row shards for the QEQ / QUAD geometries, PSGDK_INFO_NLB_MEMBER_COLS;
                                 round 6 (402): psgdk_precond_grad_apply (the parameter update fused into the apply's last product);
@@ -52,7 +53,7 @@ enum {
 };
 
 /* element types */
-enum { PSGDK_BF16 = 0, PSGDK_F32 = 1 };
+enum { PSGDK_BF16 = 0, PSGDK_F32 = 1, PSGDK_F16 = 2 /* psgdk_mx_* and psgdk_rms_norm_mx* only */ };
 /* factor kinds, psgd.py:208 */
 enum { PSGDK_DIAG = 0, PSGDK_DENSE = 1, PSGDK_SCALAR = 2 };
 /* which buffer a stage reads: the momentum EMA or the (cast) gradient, ..._ddp.py:145,150 */
@@ -377,6 +378,47 @@ int psgdk_profile_read_fused(psgdk_plan* plan, double* fused_ms, int64_t* fused_
 /* bit 1 of the same switch brackets every hot-path CALL (accumulate, update, precond_grad, apply / export) by an event pair: the summed device
  * time between the first and the last kernel of each call, i.e. the engine's kernel time per step without the host in it. */
 int psgdk_profile_read_calls(psgdk_plan* plan, double* call_ms, int64_t* calls, int reset);
+
+/* ---- microscaled (MX) numbers: the low-precision side of the layers whose weights this engine updates ------------------------------------
+ * 32 neighbours along the contracted axis share a scale 2^e (byte e + 127); an element is e2m1 (PSGDK_MX_FP4; two in a byte, the even one in the
+ * low half) or e4m3 (PSGDK_MX_FP8).  e is the smallest integer with max|x| <= L 2^e, L = 6 or 448 (nothing saturates), at least -127, 0 for a
+ * block of zeros; a block that holds an infinity or a NaN has the byte 255 and reads as NaN.  A rows x cols matrix is stored row by row, blocks
+ * along its rows, a row's codes in multiples of 256 elements (zeros behind the last), its scales in multiples of 8 bytes: psgdk_mx_storage.  The
+ * calls below read and write whole stored rows.  Codes and `work` are aligned to 16 bytes, scales to 8.  All calls are stream-ordered, allocate
+ * nothing, keep nothing and may be captured into a graph. */
+enum { PSGDK_MX_FP4 = 4, PSGDK_MX_FP8 = 8 };
+#define PSGDK_NORM_MAX_COLS 16384
+
+typedef struct {
+    const void* x;               /* rows x cols of the call's dtype, row stride ld elements */
+    const void* noise;           /* rows x cols random bytes, packed: stochastic rounding (PSGDK_MX_FP4 only); NULL: to nearest, ties to even */
+    void *codes, *scales;        /* x in MX form; NULL: not wanted */
+    void *codes_t, *scales_t;    /* x transposed (cols x rows) in MX form, blocks along x's columns; NULL: not wanted */
+    int64_t rows, cols, ld;
+} psgdk_mx_tensor;
+
+int psgdk_mx_storage(int64_t rows, int64_t cols, int fmt, int64_t* code_bytes, int64_t* scale_bytes);
+/* Rounds `count` tensors; all of them agree in which outputs and whether noise is given.  x is read once for both outputs.  Stochastic rounding goes
+ * up iff frac + (u + 1/2) / 256 >= 1, frac the distance to the lower neighbour in steps, u the element's byte (the same for both outputs). */
+int psgdk_mx_quantize(int count, const psgdk_mx_tensor* tensors, int dtype, int fmt, void* stream);
+/* out (rows x cols, packed) = the values codes and scales stand for */
+int psgdk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, int fmt, void* out, int out_dtype, void* stream);
+/* out (m x n, packed) = A B^T of A (m x k) and B (n x k), either in either format; fp32 sums, rounded once.  With an 8-bit operand the matrix
+ * instruction drops the bits of a product below 2^-13 of the largest one it adds: taken for 16-bit outputs, and for fp32 outputs where fast_sums is
+ * not 0; otherwise an fp32 output has fp32 sums throughout (at half the rate; elements below 2^-126 count as zero there).  `work`: psgdk_mx_matmul_work_bytes
+ * (0 where the contraction is not split), free for other use once the call's kernels have run. */
+int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, size_t* bytes);
+int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_fmt, const void* b_codes, const void* b_scales, int64_t n, int b_fmt,
+                    int64_t k, void* out, int out_dtype, int fast_sums, void* work, size_t work_bytes, void* stream);
+/* s = x + residual, rounded to dtype (residual NULL: s is x, nothing is written); inv = (mean of s^2 + eps)^-1/2 of every row; y = s inv gain in MX
+ * form (codes), and y transposed in MX form (codes_t); either may be NULL.  cols <= PSGDK_NORM_MAX_COLS.  s may be x or residual. */
+int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int gain_dtype, int64_t rows, int64_t cols, int dtype, float eps, int fmt,
+                      void* s, float* inv, void* codes, void* scales, void* codes_t, void* scales_t, void* stream);
+/* dx = inv (dy gain - u mean(dy gain u)) + ds with u = s inv (the gradient of x and of the residual; ds, the gradient that reaches s by its other
+ * uses, or NULL); dgain = the sum over rows of dy u, fp32, added in a fixed order.  dy has dtype or PSGDK_F32.  dx may be ds, or dy of dtype. */
+int psgdk_rms_norm_mx_backward_work_bytes(int64_t rows, int64_t cols, size_t* bytes);
+int psgdk_rms_norm_mx_backward(const void* dy, int dy_dtype, const void* s, const void* gain, int gain_dtype, const float* inv, const void* ds,
+                               int64_t rows, int64_t cols, int dtype, void* dx, float* dgain, void* work, size_t work_bytes, void* stream);
 
 /* Kernel-level test / benchmark hooks (psgdk_test_*) are declared in psgdk_test.h: exported by the same library, not part of the
  * drop-in surface. */

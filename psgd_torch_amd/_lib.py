@@ -11,10 +11,11 @@ INFO_NLB_COOP, INFO_NLB_FALLBACKS, INFO_DENSE_FACTORS, INFO_MAX_DENSE_DIM, INFO_
 INFO_NLB_MEMBER_COLS = 7
 LRA_INFO_PACKED_ROWS, LRA_INFO_GRAM_AGE = 0, 1
 BF16, F32 = 0, 1
+F16 = 2                # psgdk_mx_* and psgdk_rms_norm_mx* only
 DIAG, DENSE, SCALAR = 0, 1, 2
 GEOM_Q0P5EQ1P5, GEOM_EQ, GEOM_QEQ, GEOM_QUAD, GEOM_QEP, GEOM_QUAD4P, GEOM_PRO4P = 0, 1, 2, 3, 4, 5, 6
 SRC_EMA, SRC_GRAD = 0, 1
-ABI_VERSION = 404      # PSGDK_VERSION this binding was written against (checked at load)
+ABI_VERSION = 405      # PSGDK_VERSION this binding was written against (checked at load)
 MAX_DIMS = 26          # PSGDK_MAX_DIMS: noise pointer slots per tensor (include/psgdk.h)
 
 
@@ -32,6 +33,11 @@ class Noise(C.Structure):
 class Damp(C.Structure):
     _fields_ = [("source", C.c_int), ("damping", C.c_float), ("noise", C.POINTER(Noise)), ("seed", C.c_uint64),
                 ("offset", C.c_uint64)]
+
+
+class MxTensorArg(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("noise", C.c_void_p), ("codes", C.c_void_p), ("scales", C.c_void_p), ("codes_t", C.c_void_p),
+                ("scales_t", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64)]
 
 
 _lib = None
@@ -120,6 +126,17 @@ SIGNATURES = {
     "psgdk_lra_apply_phase": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
     "psgdk_lra_phase_segments": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int), C.POINTER(C.c_int64), C.POINTER(C.c_int),
                                            C.POINTER(C.c_int)]),
+    "psgdk_mx_storage": (C.c_int, [C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
+    "psgdk_mx_quantize": (C.c_int, [C.c_int, C.POINTER(MxTensorArg), C.c_int, C.c_int, C.c_void_p]),
+    "psgdk_mx_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
+    "psgdk_mx_matmul_work_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
+    "psgdk_mx_matmul": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_void_p,
+                                  C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "psgdk_rms_norm_mx": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_float, C.c_int, C.c_void_p,
+                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "psgdk_rms_norm_mx_backward_work_bytes": (C.c_int, [C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
+    "psgdk_rms_norm_mx_backward": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                             C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "psgdk_fill_normal": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_uint64, C.c_uint32, C.c_void_p]),
 }
 

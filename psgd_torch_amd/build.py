@@ -6,9 +6,11 @@ tree to the GPU box (it is git-ignored, not gpurun-ignored).
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "psgdk.hip")
+# two translation units, compiled side by side: the preconditioner engine, and the microscaled (MX) operators
+SRCS = [os.path.join(HERE, "csrc", "psgdk.hip"), os.path.join(HERE, "csrc", "psgdk_mx.hip")]
 OUT = os.path.join(HERE, "libpsgdk.so")
 # the measurement probes (matrix-core / HBM ceilings of the chip for bench.py's peak_measured) are a library of their own:
 # the product library carries no probe kernels
@@ -29,17 +31,33 @@ def needs_build() -> bool:
     return any(os.path.getmtime(s) > t for s in _sources())
 
 
+# (packed fp32 off in the MX unit: some forms of the packed instructions hipcc makes from plain float code have returned wrong results)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result"]
+MX_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
+def _run(cmds, verbose):
+    """Runs the commands side by side; the first that fails raises with its output."""
+    procs = []
+    for cmd in cmds:
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        procs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+    outs = [p.communicate()[0] for p in procs]
+    for p, out in zip(procs, outs):
+        if p.returncode != 0:
+            raise RuntimeError("hipcc failed:\n" + out)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return OUT
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    for src, out in ((SRC, OUT), (PROBE_SRC, PROBE_OUT)):
-        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-Wno-unused-result", src, "-o", out]
-        if verbose:
-            print(" ".join(cmd), file=sys.stderr)
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            raise RuntimeError("hipcc failed:\n" + res.stdout + res.stderr)
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in SRCS]
+        _run([[hipcc, *FLAGS, *(MX_FLAGS if s.endswith("_mx.hip") else []), "-c", s, "-o", o] for s, o in zip(SRCS, objs)]
+             + [[hipcc, *FLAGS, "-shared", PROBE_SRC, "-o", PROBE_OUT]], verbose)
+        _run([[hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", OUT]], verbose)
     return OUT
 
 

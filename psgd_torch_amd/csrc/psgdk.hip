@@ -383,6 +383,9 @@ const char* psgdk_strerror(int status) {
 
 int psgdk_last_hip_error(void) { return g_last_hip_error; }
 
+// (the library's other translation unit reports here)
+int psgdk_note_hip_error(int e) { g_last_hip_error = e; return PSGDK_ERR_HIP; }
+
 int psgdk_plan_create(psgdk_plan** out, int n_tensors, const int32_t* ndim, const int64_t* dims, double max_size,
                       double max_skew, int precond_dtype, int use_momentum) {
     if (!out || n_tensors <= 0 || !ndim || (precond_dtype != PSGDK_BF16 && precond_dtype != PSGDK_F32)) return PSGDK_ERR_INVALID;

@@ -28,6 +28,7 @@ import torch
 
 from . import _lib as L
 from .engine import KronEngine
+from .mx import refresh_mx_weights
 from .sharding import assign_owners, chunk_partition, lpt_partition, kron_step_cost, row_split_candidates
 
 
@@ -217,6 +218,25 @@ class KWNS4(torch.optim.Optimizer):
         self._split_rows = shard_split_rows is not False and self.shard_state and self.dQ in ("Q0.5EQ1.5", "Q0p5EQ1p5", "QEQ", "QUAD")
         self._split_rows_threshold = 0.5 if shard_split_rows is True else float(shard_split_rows or 0.0)
         self._rowsplit = {}
+        self._mx_weights = []        # mx.MxWeight objects renewed at the end of every step (keep_mx)
+
+    def keep_mx(self, weights) -> None:
+        """The microscaled forms of parameters this optimizer updates (mx.MxWeight), renewed from now on at the end of every step, one launch for up
+        to 32 of them: the layers of the next forward pass read weights that follow the optimizer.  Whoever else writes the parameters
+        (a checkpoint loaded into the model) calls refresh_mx_weights.  The list is not part of state_dict."""
+        from .mx import MxWeight
+        mine = {id(p) for g in self.param_groups for p in g["params"]}
+        weights = list(weights)
+        for w in weights:
+            if not isinstance(w, MxWeight):
+                raise TypeError(f"keep_mx takes MxWeight objects, got {type(w).__name__}")
+            if id(w.param) not in mine:
+                raise ValueError(f"keep_mx: the parameter of shape {tuple(w.param.shape)} is not in this optimizer's groups")
+        have = {id(w) for w in self._mx_weights}
+        for w in weights:
+            if id(w) not in have:
+                have.add(id(w))
+                self._mx_weights.append(w)
 
     # what the engine sees of a parameter: the tensors themselves here; the DTensor shell (kwns4_dtensor.py) hands over
     # the local shards (wrapped_as_torch_optimizer_for_dtensor.py:123,156)
@@ -534,6 +554,8 @@ class KWNS4(torch.optim.Optimizer):
             done_first = [it for it in items if not any(it is q for q in paused)]
             for b, sub, _, work in done_first + paused:
                 self._bucket_finish(b, group, sub, work)
+        if self._mx_weights:
+            refresh_mx_weights(self._mx_weights)
         self._global_step += 1
         left = getattr(self, "_pending_restore", None)
         if left and not getattr(self, "_restore_warned", True):

@@ -1,0 +1,470 @@
+"""Microscaled (MX) numbers next to the optimizer: the low-precision products of the layers whose weights KWNS4 updates, and the norm before them.
+
+    mx_quantize, mx_dequantize                 rounding to 4 or 8 bits with a scale per 32 neighbours, and back
+    mx_matmul                                  A B^T of two MX matrices on the scaled matrix instructions, fp32 sums
+    rms_norm_mx, rms_norm_mx_backward          residual addition + root-mean-square norm ending in MX blocks; its gradients
+    MxWeight, mx_linear, mx_norm_linear        a weight kept in MX form in both directions, and differentiable layers on it
+    refresh_mx_weights, KWNS4.keep_mx          the kept forms renewed from the parameters, by hand or at the end of every optimizer step
+
+The format (include/psgdk.h): 32 neighbours along the contracted axis share a scale 2^e (byte e + 127); an element is e2m1 ("fp4") or e4m3 ("fp8").
+e is the smallest integer that keeps the block's largest magnitude inside the element's range (6 or 448), so nothing saturates; a block with an
+infinity or a NaN reads as NaN.  Rows are stored in multiples of 256 elements.
+
+Everything computes through libpsgdk.so on the current stream of the tensors' device; there is no CPU fallback.  No call keeps or reuses memory of its
+own: outputs and workspaces come from torch's allocator, so calls on different streams, in captured graphs and on several devices do not meet.
+A CUDA graph of a backward pass must not be captured while another autograd graph over the same leaves is alive (torch binds a leaf's gradient
+accumulation to the stream it first ran on, and a capture that has to wait for that stream fails): free earlier losses first, or use
+torch.autograd.grad inside the capture.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib as L
+
+_FMT = {"fp4": 4, "fp8": 8}
+_DTYPE = {torch.bfloat16: L.BF16, torch.float32: L.F32, torch.float16: L.F16}
+_PAD = 256          # elements a stored row is a multiple of
+_BLOCK = 32
+NORM_MAX_COLS = 16384
+
+
+def _bad(msg):
+    return L.PsgdkError(L.PSGDK_ERR_INVALID, msg)
+
+
+def _fmt(fmt) -> int:
+    if fmt not in _FMT:
+        raise _bad(f'MX format {fmt!r}: "fp4" (e2m1) or "fp8" (e4m3)')
+    return _FMT[fmt]
+
+
+def _dtype(what, dt) -> int:
+    if dt not in _DTYPE:
+        raise _bad(f"{what} has dtype {dt}: bfloat16, float16 or float32")
+    return _DTYPE[dt]
+
+
+def _tensor(what, t, device=None):
+    if not isinstance(t, torch.Tensor):
+        raise _bad(f"{what} is not a tensor")
+    if t.device.type != "cuda":
+        raise _bad(f"{what} lives on {t.device}: MX operators need tensors on a ROCm device; there is no CPU fallback")
+    if device is not None and t.device != device:
+        raise _bad(f"{what} lives on {t.device}, the others on {device}")
+
+
+def _rows(what, x) -> torch.Tensor:
+    """x as a matrix of rows with contiguous elements (a view where the strides allow it, a copy otherwise)."""
+    if x.dim() == 0:
+        raise _bad(f"{what} has no dimensions: MX blocks run along the last one")
+    if x.dim() != 2:
+        n = 1
+        for d in x.shape[:-1]:
+            n *= d
+        x = x.reshape(n, x.shape[-1])
+    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    return x
+
+
+def _ld(x) -> int:
+    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+
+
+def _ptr(t) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+class _on:
+    """The device of `t` current, and its current stream as a pointer."""
+
+    def __init__(self, t):
+        self.guard = torch.cuda.device(t.device)
+        self.device = t.device
+
+    def __enter__(self):
+        self.guard.__enter__()
+        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def __exit__(self, *a):
+        return self.guard.__exit__(*a)
+
+
+class MxTensor:
+    """A rows x cols matrix in MX form, blocks along its rows.  codes: uint8 (rows, pad(cols) * bits / 8), in 4 bits the even element in the low half
+    of its byte; scales: uint8 (rows, pad(cols) / 32), 2^(byte - 127), 255 for NaN; pad: the next multiple of 256.  Elements behind `cols` are zero
+    codes (they take part in products).  Holds no autograd history."""
+
+    __slots__ = ("codes", "scales", "shape", "fmt")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, int], fmt: str):
+        bits = _fmt(fmt)
+        rows, cols = (int(d) for d in shape)
+        if rows < 0 or cols < 0:
+            raise _bad(f"MxTensor shape {tuple(shape)}")
+        wide = -(-cols // _PAD) * _PAD
+        for what, t, n in (("codes", codes, wide * bits // 8), ("scales", scales, wide // _BLOCK)):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or tuple(t.shape) != (rows, n) or not t.is_contiguous():
+                raise _bad(f"MxTensor {what}: a contiguous uint8 tensor of shape {(rows, n)} for a {rows} x {cols} matrix in {fmt}")
+        if codes.device != scales.device:
+            raise _bad(f"MxTensor codes live on {codes.device}, scales on {scales.device}")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 8:
+            raise _bad("MxTensor codes need 16-byte, scales 8-byte alignment")
+        self.codes, self.scales, self.shape, self.fmt = codes, scales, (rows, cols), fmt
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, fmt: str, device) -> "MxTensor":
+        wide = -(-cols // _PAD) * _PAD
+        return cls(torch.empty((rows, wide * _fmt(fmt) // 8), dtype=torch.uint8, device=device),
+                   torch.empty((rows, wide // _BLOCK), dtype=torch.uint8, device=device), (rows, cols), fmt)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
+        return mx_dequantize(self, dtype)
+
+    def __repr__(self):
+        return f"MxTensor({self.shape[0]} x {self.shape[1]}, {self.fmt}, {self.device})"
+
+
+def _mx(what, t, device=None) -> MxTensor:
+    if not isinstance(t, MxTensor):
+        raise _bad(f"{what} is not an MxTensor")
+    _tensor(what, t.codes, device)
+    return t
+
+
+# ---------------------------------------------------------------------------------------------------------------------------- rounding
+
+def _quantize(items, fmt, which, stream):
+    """items: [(x (2-D), noise or None, MxTensor of x or None, MxTensor of x transposed or None)] of one dtype."""
+    jobs = (L.MxTensorArg * len(items))()
+    for j, (x, noise, r, c) in zip(jobs, items):
+        j.x, j.noise, j.rows, j.cols, j.ld = _ptr(x), _ptr(noise), x.shape[0], x.shape[1], _ld(x)
+        if r is not None:
+            j.codes, j.scales = _ptr(r.codes), _ptr(r.scales)
+        if c is not None:
+            j.codes_t, j.scales_t = _ptr(c.codes), _ptr(c.scales)
+    L.check(L.lib().psgdk_mx_quantize(len(items), jobs, _DTYPE[items[0][0].dtype], _FMT[fmt], stream), "mx_quantize")
+
+
+def mx_quantize(x: torch.Tensor, fmt: str = "fp4", *, which: str = "rows", noise: Optional[torch.Tensor] = None):
+    """x (..., K) in bf16, fp16 or fp32 -> MX form.  which: "rows" -- x as an (R x K) matrix, blocks along K; "cols" -- its transpose (K x R), blocks
+    along R; "both" -- the pair, from one reading of x.  Rounds to nearest, ties to even; with `noise` (uint8, x's shape, uniform bytes; "fp4" only)
+    stochastically: up iff frac + (noise + 1/2) / 256 >= 1, the same byte for both directions.  The result carries no gradient."""
+    _tensor("x", x)
+    _dtype("x", x.dtype)
+    _fmt(fmt)
+    if which not in ("rows", "cols", "both"):
+        raise _bad(f'which={which!r}: "rows", "cols" or "both"')
+    shape = x.shape
+    x = _rows("x", x.detach())
+    if noise is not None:
+        if fmt != "fp4":
+            raise _bad("stochastic rounding is for fp4: an 8-bit element is rounded to nearest")
+        _tensor("noise", noise, x.device)
+        if noise.dtype != torch.uint8 or noise.shape != shape:
+            raise _bad(f"noise: uint8 of x's shape {tuple(shape)}, got {noise.dtype} {tuple(noise.shape)}")
+        noise = noise.contiguous()
+    rows, cols = x.shape
+    r = MxTensor.empty(rows, cols, fmt, x.device) if which != "cols" else None
+    c = MxTensor.empty(cols, rows, fmt, x.device) if which != "rows" else None
+    with _on(x) as stream:
+        _quantize([(x, noise, r, c)], fmt, which, stream)
+    return (r, c) if which == "both" else r if c is None else c
+
+
+def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values t stands for (bf16 and fp32 hold them exactly within their range)."""
+    _mx("t", t)
+    out = torch.empty(t.shape, dtype=dtype, device=t.device)
+    code = _dtype("out", dtype)
+    with _on(out) as stream:
+        L.check(L.lib().psgdk_mx_dequantize(_ptr(t.codes), _ptr(t.scales), *t.shape, _FMT[t.fmt], _ptr(out), code, stream), "mx_dequantize")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------------------- products
+
+def mx_matmul(a: MxTensor, b: MxTensor, *, out_dtype: torch.dtype = torch.bfloat16, fast_sums: bool = False) -> torch.Tensor:
+    """A B^T (M x N) of a (M x K) and b (N x K), either in either format; fp32 sums, rounded once to out_dtype.  The same inputs give the same bits:
+    a long contraction with few outputs is split, and the parts are added in a fixed order.
+    With an fp8 operand the scaled matrix instruction drops the bits of a product below 2^-13 of the largest one it adds (about 2e-5 of a result):
+    that is taken for 16-bit outputs, whose own rounding is a hundred times larger, and for fp32 outputs with fast_sums=True; an fp32 output has
+    fp32 sums throughout otherwise, at half the rate (elements below 2^-126 count as zero there)."""
+    _mx("a", a)
+    _mx("b", b, a.device)
+    if a.shape[1] != b.shape[1]:
+        raise _bad(f"mx_matmul: a is {a.shape[0]} x {a.shape[1]}, b is {b.shape[0]} x {b.shape[1]}: both are contracted along their rows")
+    code = _dtype("out", out_dtype)
+    (m, k), n = a.shape, b.shape[0]
+    out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+    lib = L.lib()
+    wb = C.c_size_t()
+    L.check(lib.psgdk_mx_matmul_work_bytes(m, n, k, C.byref(wb)), "mx_matmul_work_bytes")
+    work = torch.empty(wb.value, dtype=torch.uint8, device=a.device) if wb.value else None
+    with _on(out) as stream:
+        L.check(lib.psgdk_mx_matmul(_ptr(a.codes), _ptr(a.scales), m, _FMT[a.fmt], _ptr(b.codes), _ptr(b.scales), n, _FMT[b.fmt], k, _ptr(out), code,
+                                    int(bool(fast_sums)), _ptr(work), wb.value, stream), "mx_matmul")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------------------------- norm
+
+def _norm_args(x, gain, residual):
+    _tensor("x", x)
+    _dtype("x", x.dtype)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise _bad(f"x of shape {tuple(x.shape)}: the norm needs at least one column")
+    if x.shape[-1] > NORM_MAX_COLS:
+        raise L.PsgdkError(L.PSGDK_ERR_UNSUPPORTED, f"rms_norm_mx: {x.shape[-1]} columns, at most {NORM_MAX_COLS} (a row stays in registers)")
+    _tensor("gain", gain, x.device)
+    _dtype("gain", gain.dtype)
+    if gain.shape != x.shape[-1:]:
+        raise _bad(f"gain of shape {tuple(gain.shape)} for rows of {x.shape[-1]}")
+    if residual is not None:
+        _tensor("residual", residual, x.device)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise _bad(f"residual is {residual.dtype} {tuple(residual.shape)}, x is {x.dtype} {tuple(x.shape)}")
+
+
+def rms_norm_mx(x: torch.Tensor, gain: torch.Tensor, residual: Optional[torch.Tensor] = None, *, eps: float = 1e-5, fmt: str = "fp8",
+                which: str = "rows"):
+    """s = x + residual (rounded to x's dtype; without a residual s is x), inv = (mean of s^2 + eps)^-1/2 of every row in fp32, y = s inv gain.
+    Returns (y in MX form as mx_quantize's `which` says, s, inv).  y is rounded once, from fp32.  At most 16384 columns.  Not differentiable by
+    itself (rms_norm_mx_backward has the gradients, mx_norm_linear is the differentiable layer)."""
+    _norm_args(x, gain, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or gain.requires_grad or residual is not None and residual.requires_grad):
+        raise _bad("rms_norm_mx does not record gradients: use mx_norm_linear, or call it under torch.no_grad()")
+    bits = _fmt(fmt)
+    if which not in ("rows", "cols", "both"):
+        raise _bad(f'which={which!r}: "rows", "cols" or "both"')
+    if not 0.0 <= eps < float("inf"):
+        raise _bad(f"eps={eps}")
+    shape = x.shape
+    d = shape[-1]
+    x2, res = x.contiguous(), None if residual is None else residual.contiguous()
+    s = x2 if res is None else torch.empty_like(x2)
+    n = x2.numel() // d
+    inv = torch.empty(n, dtype=torch.float32, device=x.device)
+    r = MxTensor.empty(n, d, fmt, x.device) if which != "cols" else None
+    c = MxTensor.empty(d, n, fmt, x.device) if which != "rows" else None
+    gain = gain.contiguous()
+    with _on(x2) as stream:
+        L.check(L.lib().psgdk_rms_norm_mx(_ptr(x2), _ptr(res), _ptr(gain), _DTYPE[gain.dtype], n, d, _DTYPE[x.dtype], float(eps), bits,
+                                          _ptr(s), _ptr(inv), r and _ptr(r.codes), r and _ptr(r.scales), c and _ptr(c.codes), c and _ptr(c.scales),
+                                          stream), "rms_norm_mx")
+    y = (r, c) if which == "both" else r if c is None else c
+    return y, s, inv
+
+
+def rms_norm_mx_backward(dy: torch.Tensor, s: torch.Tensor, gain: torch.Tensor, inv: torch.Tensor, *, ds: Optional[torch.Tensor] = None):
+    """(dx, dgain) of rms_norm_mx at the s and inv it returned, the rounding of y taken as the identity: with u = s inv,
+    dx = inv (dy gain - u mean(dy gain u)) + ds -- the gradient of x and of the residual -- and dgain = the sum over rows of dy u (fp32, the same
+    bits every run).  dy: s's dtype or fp32.  ds: the gradient that reaches s by its other uses."""
+    _norm_args(s, gain, ds)
+    _tensor("dy", dy, s.device)
+    _tensor("inv", inv, s.device)
+    if dy.shape != s.shape or dy.dtype not in (s.dtype, torch.float32):
+        raise _bad(f"dy is {dy.dtype} {tuple(dy.shape)}, s is {s.dtype} {tuple(s.shape)}: the same shape, the same dtype or float32")
+    d = s.shape[-1]
+    n = s.numel() // d
+    if inv.dtype != torch.float32 or inv.numel() != n:
+        raise _bad(f"inv: {n} values in float32, got {inv.dtype} {tuple(inv.shape)}")
+    dy, s, gain, inv = dy.contiguous(), s.contiguous(), gain.contiguous(), inv.contiguous()
+    ds = None if ds is None else ds.contiguous()
+    dx = torch.empty_like(s)
+    dgain = torch.empty(d, dtype=torch.float32, device=s.device)
+    lib = L.lib()
+    wb = C.c_size_t()
+    L.check(lib.psgdk_rms_norm_mx_backward_work_bytes(n, d, C.byref(wb)), "rms_norm_mx_backward_work_bytes")
+    work = torch.empty(max(wb.value, 4), dtype=torch.uint8, device=s.device)
+    with _on(s) as stream:
+        L.check(lib.psgdk_rms_norm_mx_backward(_ptr(dy), _DTYPE[dy.dtype], _ptr(s), _ptr(gain), _DTYPE[gain.dtype], _ptr(inv), _ptr(ds), n, d,
+                                               _DTYPE[s.dtype], _ptr(dx), _ptr(dgain), _ptr(work), wb.value, stream), "rms_norm_mx_backward")
+    return dx, dgain
+
+
+# ---------------------------------------------------------------------------------------------------------------------------- layers
+
+class MxWeight:
+    """The MX forms of a 2-D parameter (N x K): `rows` (blocks along K: the forward product) and `cols` (the transpose, blocks along N: the gradient of
+    the layer's input).  They are rounded once here and renewed by refresh() -- KWNS4.keep_mx does that after every step.  `rows` / `cols` may be
+    handed over instead; backward=False keeps the forward form only."""
+
+    def __init__(self, param: torch.Tensor, fmt: str = "fp4", *, backward: bool = True, rows: Optional[MxTensor] = None, cols: Optional[MxTensor] = None):
+        _tensor("param", param)
+        _dtype("param", param.dtype)
+        if param.dim() != 2:
+            raise _bad(f"MxWeight holds a matrix, got shape {tuple(param.shape)}")
+        if type(param) not in (torch.Tensor, torch.nn.Parameter):
+            raise _bad(f"MxWeight holds a plain tensor or parameter, got {type(param).__name__}")
+        n, k = param.shape
+        for what, t, shape in (("rows", rows, (n, k)), ("cols", cols, (k, n))):
+            if t is not None and _mx(what, t, param.device).shape != shape:
+                raise _bad(f"MxWeight {what} is {t.shape[0]} x {t.shape[1]}, expected {shape[0]} x {shape[1]}")
+        self.param = param
+        self.fmt = rows.fmt if rows is not None else fmt
+        _fmt(self.fmt)
+        if cols is not None and cols.fmt != self.fmt:
+            raise _bad(f"MxWeight rows are {self.fmt}, cols {cols.fmt}")
+        given = rows is not None
+        self.rows = rows if given else MxTensor.empty(n, k, self.fmt, param.device)
+        self.cols = cols if cols is not None else MxTensor.empty(k, n, self.fmt, param.device) if backward and not given else None
+        if not given:
+            self.refresh()
+
+    def refresh(self):
+        refresh_mx_weights([self])
+
+
+@torch.no_grad()
+def refresh_mx_weights(weights: Sequence[MxWeight]) -> None:
+    """Rounds the parameters of `weights` again into the memory of their MX forms, one launch for up to 32 of them: what KWNS4 does at the end of a step for
+    the weights it keeps.  An autograd graph that was recorded before and still needs the old forms refuses its backward pass, as for any tensor
+    that was modified in place."""
+    groups = {}
+    for w in weights:
+        if not isinstance(w, MxWeight):
+            raise _bad(f"{type(w).__name__} is not an MxWeight")
+        p = w.param.detach()
+        _tensor("param", p, w.rows.device)
+        _dtype("param", p.dtype)
+        if tuple(p.shape) != w.rows.shape:
+            raise _bad(f"the parameter is {tuple(p.shape)} now, its MxWeight {w.rows.shape}")
+        groups.setdefault((p.device, p.dtype, w.fmt, w.cols is not None), []).append((_rows("param", p), None, w.rows, w.cols))
+    for (device, _, fmt, both), items in groups.items():
+        with _on(items[0][0]) as stream:
+            _quantize(items, fmt, "both" if both else "rows", stream)
+        for _, _, r, c in items:
+            torch.autograd.graph.increment_version([t for q in (r, c) if q is not None for t in (q.codes, q.scales)])
+
+
+def _restore(ctx, i, shape, fmt) -> MxTensor:
+    codes, scales = ctx.saved_tensors[i:i + 2]
+    return MxTensor(codes, scales, shape, fmt)
+
+
+def _weight_args(x, weight, fmt, grad_fmt):
+    if not isinstance(weight, MxWeight):
+        raise _bad(f"weight is a {type(weight).__name__}, not an MxWeight")
+    _tensor("x", x, weight.rows.device)
+    _dtype("x", x.dtype)
+    _fmt(fmt)
+    _fmt(grad_fmt)
+    if x.dim() == 0 or x.shape[-1] != weight.rows.shape[1]:
+        raise _bad(f"x of shape {tuple(x.shape)} against a weight of {weight.rows.shape}")
+
+
+def _need_cols(weight):
+    if weight.cols is None:
+        raise _bad("the input of this layer needs a gradient: MxWeight(..., backward=True) keeps the form that its product reads")
+
+
+def _tracked(*ts):
+    """The tensors as autograd is to see them: without gradient mode none of them needs one (a custom function is told of requires_grad alone)."""
+    return ts if torch.is_grad_enabled() else tuple(None if t is None else t.detach() for t in ts)
+
+
+def _product_grads(ctx, dout, need_x, need_w, cols_at, act_at, x_dtype):
+    """(gradient of the product's input in x_dtype, of the weight) from dout."""
+    n, k = ctx.weight_shape
+    d2 = _rows("gradient", dout)
+    which = "both" if need_x and need_w else "rows" if need_x else "cols"
+    q = mx_quantize(d2, ctx.grad_fmt, which=which)
+    dr, dc = q if which == "both" else (q, None) if need_x else (None, q)
+    dx = mx_matmul(dr, _restore(ctx, cols_at, (k, n), ctx.weight_fmt), out_dtype=x_dtype, fast_sums=True) if need_x else None
+    dw = mx_matmul(dc, _restore(ctx, act_at, (k, d2.shape[0]), ctx.fmt), out_dtype=ctx.weight_dtype, fast_sums=True) if need_w else None
+    return dx, dw
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, param, weight, fmt, grad_fmt):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        xr = mx_quantize(x, fmt, which="both" if need_w else "rows")
+        xr, xc = xr if need_w else (xr, None)
+        out = mx_matmul(xr, weight.rows, out_dtype=x.dtype, fast_sums=True)
+        saved = []
+        if need_x:
+            _need_cols(weight)
+            saved += [weight.cols.codes, weight.cols.scales]
+        if need_w:
+            saved += [xc.codes, xc.scales]
+        ctx.save_for_backward(*saved)
+        ctx.weight_shape, ctx.weight_fmt, ctx.weight_dtype, ctx.fmt, ctx.grad_fmt = weight.rows.shape, weight.fmt, param.dtype, fmt, grad_fmt
+        ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
+        return out.view(*x.shape[:-1], weight.rows.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        dx, dw = _product_grads(ctx, dout, need_x, need_w, 0, 2 if need_x else 0, ctx.x_dtype)
+        return (dx.view(ctx.x_shape) if need_x else None), dw, None, None, None
+
+
+class _NormLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, gain, param, weight, eps, fmt, grad_fmt):
+        need_s = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        need_g, need_w = ctx.needs_input_grad[2:4]
+        y, s, inv = rms_norm_mx(x, gain, residual, eps=eps, fmt=fmt, which="both" if need_w else "rows")
+        yr, yc = y if need_w else (y, None)
+        out = mx_matmul(yr, weight.rows, out_dtype=x.dtype, fast_sums=True)
+        saved = [s, inv, gain]
+        if need_s or need_g:
+            _need_cols(weight)
+            saved += [weight.cols.codes, weight.cols.scales]
+        if need_w:
+            saved += [yc.codes, yc.scales]
+        ctx.save_for_backward(*saved)
+        ctx.weight_shape, ctx.weight_fmt, ctx.weight_dtype, ctx.fmt, ctx.grad_fmt = weight.rows.shape, weight.fmt, param.dtype, fmt, grad_fmt
+        ctx.set_materialize_grads(False)
+        out = out.view(*x.shape[:-1], weight.rows.shape[0])
+        return out if residual is None else (out, s)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, ds=None):
+        need_s = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        need_g, need_w = ctx.needs_input_grad[2:4]
+        need_y = need_s or need_g
+        s, inv, gain = ctx.saved_tensors[:3]
+        dx = dg = dw = None
+        if dout is not None:
+            # (the gradient of y stays in fp32 between the two kernels: one rounding, at dx)
+            dy, dw = _product_grads(ctx, dout, need_y, need_w, 3, 5 if need_y else 3, torch.float32)
+            if need_y:
+                dx, dg = rms_norm_mx_backward(dy.view(s.shape), s, gain, inv, ds=ds)
+                dg = dg.to(gain.dtype)
+        elif need_s:
+            dx = ds
+        need = ctx.needs_input_grad
+        return (dx if need[0] else None), (dx if need[1] else None), (dg if need_g else None), dw, None, None, None, None
+
+
+def mx_linear(x: torch.Tensor, weight: MxWeight, *, fmt: str = "fp8", grad_fmt: str = "fp8") -> torch.Tensor:
+    """x W^T in x's dtype: x is rounded to `fmt`, W is the weight's kept form.  Backward: dx = MX(dY) W and dW = MX(dY^T) MX(x^T)^T with dY rounded to
+    `grad_fmt` along the contracted axis of each (roundings count as the identity); dW has the parameter's dtype.  The products take
+    mx_matmul's fast_sums: their operands are rounded to 4 significant bits at best."""
+    _weight_args(x, weight, fmt, grad_fmt)
+    x, param = _tracked(x, weight.param)
+    return _Linear.apply(x, param, weight, fmt, grad_fmt)
+
+
+def mx_norm_linear(x: torch.Tensor, gain: torch.Tensor, weight: MxWeight, residual: Optional[torch.Tensor] = None, *, eps: float = 1e-5,
+                   fmt: str = "fp8", grad_fmt: str = "fp8"):
+    """(rms_norm(x + residual) W^T, s): the residual's addition, the norm that ends in MX blocks and the product that reads them, differentiable in x,
+    residual, gain and the weight's parameter.  s = x + residual is the next residual (x itself without one)."""
+    _weight_args(x, weight, fmt, grad_fmt)
+    _norm_args(x, gain, residual)
+    x, residual, gain, param = _tracked(x, residual, gain, weight.param)
+    out = _NormLinear.apply(x, residual, gain, param, weight, eps, fmt, grad_fmt)
+    return (out, x) if residual is None else out
