@@ -129,9 +129,9 @@ SIGNATURES = {
     "psgdk_mx_storage": (C.c_int, [C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     "psgdk_mx_quantize": (C.c_int, [C.c_int, C.POINTER(MxTensorArg), C.c_int, C.c_int, C.c_void_p]),
     "psgdk_mx_dequantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
-    "psgdk_mx_matmul_work_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),
+    "psgdk_mx_matmul_work_bytes": (C.c_int, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
     "psgdk_mx_matmul": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_int64, C.c_void_p,
-                                  C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+                                  C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "psgdk_rms_norm_mx": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int, C.c_float, C.c_int, C.c_void_p,
                                     C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "psgdk_rms_norm_mx_backward_work_bytes": (C.c_int, [C.c_int64, C.c_int64, C.POINTER(C.c_size_t)]),

@@ -14,6 +14,8 @@ extern "C" int psgdk_note_hip_error(int e);      // psgdk.hip: what psgdk_last_h
 #define MX_LAUNCHED() MX_HIPCHK(hipGetLastError())
 
 static const int64_t kMaxDim = (1ll << 31) - 65536;      // rows and columns are 32-bit in the kernels; offsets are 64-bit
+static const int64_t kMaxN = 1ll << 22;                  // a product's columns: 256 rows of the output lie within 32-bit offsets
+static const int64_t kMaxK = 1ll << 23;                  // a product's contraction: 256 stored rows of an operand tile lie within 32-bit offsets
 
 static bool mx_fmt_ok(int f) { return f == PSGDK_MX_FP4 || f == PSGDK_MX_FP8; }
 static bool mx_dtype_ok(int d) { return d == PSGDK_BF16 || d == PSGDK_F32 || d == PSGDK_F16; }
@@ -79,8 +81,10 @@ static int mx_back_lines(int64_t rows, int64_t cols) {
 }
 
 // ---- products ----------------------------------------------------------------------------------------------------------------------------
+// a 32-bit output with an 8-bit operand: fp32 sums through bf16 products (gemm_mx.hiph)
+static bool mx_wide(int a_fmt, int b_fmt, int out_dtype) { return out_dtype == PSGDK_F32 && (a_fmt == PSGDK_MX_FP8 || b_fmt == PSGDK_MX_FP8); }
 struct MxPlan { bool skinny; int mt, nt, bm, bn, splits; };
-static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS) {
+static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, bool wide) {
     MxPlan p{};
     p.splits = 1;
     if (M <= 64) {
@@ -90,7 +94,7 @@ static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS) {
         return p;
     }
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    p.bm = p.bn = big >= 256 ? 256 : 128;
+    p.bm = p.bn = big >= 256 && !wide ? 256 : 128;
     const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
     while (p.splits < 16 && tiles * p.splits * 2 <= 512 && KS / (p.splits * 2) >= 2) p.splits *= 2;
     return p;
@@ -105,8 +109,8 @@ static int mx_launch_product(const MxGemm& g, const MxPlan& p, hipStream_t st) {
 #undef MX_SKINNY
     } else {
         const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
-        if (p.bm == 256) mx_tile_gemm_kernel<FA, FB, WIDE, 256, 256, 128, 64><<<grid, 512, 0, st>>>(g);
-        else mx_tile_gemm_kernel<FA, FB, WIDE, 128, 128, 64, 64><<<grid, 256, 0, st>>>(g);
+        if constexpr (!WIDE) if (p.bm == 256) mx_tile_gemm_kernel<FA, FB, WIDE, 256, 256><<<grid, 256, 0, st>>>(g);
+        if (p.bm == 128) mx_tile_gemm_kernel<FA, FB, WIDE, 128, 128><<<grid, 256, 0, st>>>(g);
     }
     MX_LAUNCHED();
     if (g.part) {
@@ -195,23 +199,26 @@ int psgdk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int
     });
 }
 
-int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, size_t* bytes) {
+int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int out_dtype, size_t* bytes) {
     if (m < 0 || n < 0 || k < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim || !bytes) return PSGDK_ERR_INVALID;
-    const MxPlan p = mx_plan(m, n, mx_pad(k) / MX_PAD);
+    if (!mx_fmt_ok(a_fmt) || !mx_fmt_ok(b_fmt) || !mx_dtype_ok(out_dtype)) return PSGDK_ERR_INVALID;
+    const MxPlan p = mx_plan(m, n, mx_pad(k) / MX_PAD, mx_wide(a_fmt, b_fmt, out_dtype));
     *bytes = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
     return PSGDK_OK;
 }
 
 int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_fmt, const void* b_codes, const void* b_scales, int64_t n, int b_fmt,
-                    int64_t k, void* out, int out_dtype, int fast_sums, void* work, size_t work_bytes, void* stream) {
+                    int64_t k, void* out, int out_dtype, void* work, size_t work_bytes, void* stream) {
     if (m < 0 || n < 0 || k < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim) return PSGDK_ERR_INVALID;
     if (!mx_fmt_ok(a_fmt) || !mx_fmt_ok(b_fmt) || !mx_dtype_ok(out_dtype)) return PSGDK_ERR_INVALID;
+    if (k > kMaxK || n > kMaxN) return PSGDK_ERR_UNSUPPORTED;
     if (m == 0 || n == 0) return PSGDK_OK;
     if (!out || !mx_aligned(out, mx_size(out_dtype))) return PSGDK_ERR_INVALID;
     if (k > 0 && (!a_codes || !a_scales || !b_codes || !b_scales)) return PSGDK_ERR_INVALID;
     if (!mx_aligned(a_codes, 16) || !mx_aligned(b_codes, 16) || !mx_aligned(a_scales, 8) || !mx_aligned(b_scales, 8)) return PSGDK_ERR_INVALID;
     const int64_t KS = mx_pad(k) / MX_PAD;
-    const MxPlan p = mx_plan(m, n, KS);
+    const bool wide = mx_wide(a_fmt, b_fmt, out_dtype);
+    const MxPlan p = mx_plan(m, n, KS, wide);
     const size_t need = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
     if (need && (!work || work_bytes < need || !mx_aligned(work, 16))) return PSGDK_ERR_INVALID;
     const int64_t tm = p.skinny ? 1 : (m + p.bm - 1) / p.bm, tn = p.skinny ? 1 : (n + p.bn - 1) / p.bn;
@@ -220,7 +227,7 @@ int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_
                    (int)m, (int)n, (int)KS, out_dtype, p.splits, (int)tm, (int)tn};
     const hipStream_t st = (hipStream_t)stream;
     if (a_fmt == PSGDK_MX_FP4 && b_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 4, false>(g, p, st);
-    if (out_dtype == PSGDK_F32 && !fast_sums) {
+    if (wide) {
         if (a_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 8, true>(g, p, st);
         return b_fmt == PSGDK_MX_FP4 ? mx_launch_product<8, 4, true>(g, p, st) : mx_launch_product<8, 8, true>(g, p, st);
     }

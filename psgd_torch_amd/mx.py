@@ -19,6 +19,7 @@ torch.autograd.grad inside the capture.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -51,7 +52,7 @@ def _dtype(what, dt) -> int:
 def _tensor(what, t, device=None):
     if not isinstance(t, torch.Tensor):
         raise _bad(f"{what} is not a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise _bad(f"{what} lives on {t.device}: MX operators need tensors on a ROCm device; there is no CPU fallback")
     if device is not None and t.device != device:
         raise _bad(f"{what} lives on {t.device}, the others on {device}")
@@ -79,19 +80,28 @@ def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-class _on:
-    """The device of `t` current, and its current stream as a pointer."""
+# (the calls below cost microseconds on the device at the smallest sizes: the host side avoids objects it does not need)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    def __init__(self, t):
-        self.guard = torch.cuda.device(t.device)
-        self.device = t.device
 
-    def __enter__(self):
-        self.guard.__enter__()
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+def _launch(what, device, fn, *args):
+    """fn(*args, current stream of `device`) with that device current."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        L.check(rc, what)
 
-    def __exit__(self, *a):
-        return self.guard.__exit__(*a)
+
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(name, *sizes) -> int:
+    """The library's answer for these sizes (it depends on nothing else)."""
+    wb = C.c_size_t()
+    L.check(getattr(L.lib(), name)(*sizes, C.byref(wb)), name)
+    return wb.value
 
 
 class MxTensor:
@@ -119,8 +129,15 @@ class MxTensor:
     @classmethod
     def empty(cls, rows: int, cols: int, fmt: str, device) -> "MxTensor":
         wide = -(-cols // _PAD) * _PAD
-        return cls(torch.empty((rows, wide * _fmt(fmt) // 8), dtype=torch.uint8, device=device),
-                   torch.empty((rows, wide // _BLOCK), dtype=torch.uint8, device=device), (rows, cols), fmt)
+        return cls._of(torch.empty((rows, wide * _fmt(fmt) // 8), dtype=torch.uint8, device=device),
+                       torch.empty((rows, wide // _BLOCK), dtype=torch.uint8, device=device), (rows, cols), fmt)
+
+    @classmethod
+    def _of(cls, codes, scales, shape, fmt) -> "MxTensor":
+        """From parts that are known to fit."""
+        t = object.__new__(cls)
+        t.codes, t.scales, t.shape, t.fmt = codes, scales, shape, fmt
+        return t
 
     @property
     def device(self):
@@ -142,16 +159,27 @@ def _mx(what, t, device=None) -> MxTensor:
 
 # ---------------------------------------------------------------------------------------------------------------------------- rounding
 
-def _quantize(items, fmt, which, stream):
-    """items: [(x (2-D), noise or None, MxTensor of x or None, MxTensor of x transposed or None)] of one dtype."""
+def _quantize(items, fmt, device):
+    """items: [(x (2-D), noise or None, MxTensor of x or None, MxTensor of x transposed or None)] of one dtype, all with the same outputs."""
     jobs = (L.MxTensorArg * len(items))()
     for j, (x, noise, r, c) in zip(jobs, items):
-        j.x, j.noise, j.rows, j.cols, j.ld = _ptr(x), _ptr(noise), x.shape[0], x.shape[1], _ld(x)
+        j.x, j.rows, j.cols, j.ld = x.data_ptr(), x.shape[0], x.shape[1], _ld(x)
+        if noise is not None:
+            j.noise = noise.data_ptr()
         if r is not None:
-            j.codes, j.scales = _ptr(r.codes), _ptr(r.scales)
+            j.codes, j.scales = r.codes.data_ptr(), r.scales.data_ptr()
         if c is not None:
-            j.codes_t, j.scales_t = _ptr(c.codes), _ptr(c.scales)
-    L.check(L.lib().psgdk_mx_quantize(len(items), jobs, _DTYPE[items[0][0].dtype], _FMT[fmt], stream), "mx_quantize")
+            j.codes_t, j.scales_t = c.codes.data_ptr(), c.scales.data_ptr()
+    _launch("mx_quantize", device, L.lib().psgdk_mx_quantize, len(items), jobs, _DTYPE[items[0][0].dtype], _FMT[fmt])
+
+
+def _rounded(x, fmt, rows, cols, noise=None):
+    """(MxTensor of x or None, MxTensor of x transposed or None) of a checked tensor."""
+    n, k = x.shape
+    r = MxTensor.empty(n, k, fmt, x.device) if rows else None
+    c = MxTensor.empty(k, n, fmt, x.device) if cols else None
+    _quantize([(x, noise, r, c)], fmt, x.device)
+    return r, c
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "fp4", *, which: str = "rows", noise: Optional[torch.Tensor] = None):
@@ -164,7 +192,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "fp4", *, which: str = "rows", noise
     if which not in ("rows", "cols", "both"):
         raise _bad(f'which={which!r}: "rows", "cols" or "both"')
     shape = x.shape
-    x = _rows("x", x.detach())
+    x = _rows("x", x.detach() if x.requires_grad else x)
     if noise is not None:
         if fmt != "fp4":
             raise _bad("stochastic rounding is for fp4: an 8-bit element is rounded to nearest")
@@ -172,46 +200,42 @@ def mx_quantize(x: torch.Tensor, fmt: str = "fp4", *, which: str = "rows", noise
         if noise.dtype != torch.uint8 or noise.shape != shape:
             raise _bad(f"noise: uint8 of x's shape {tuple(shape)}, got {noise.dtype} {tuple(noise.shape)}")
         noise = noise.contiguous()
-    rows, cols = x.shape
-    r = MxTensor.empty(rows, cols, fmt, x.device) if which != "cols" else None
-    c = MxTensor.empty(cols, rows, fmt, x.device) if which != "rows" else None
-    with _on(x) as stream:
-        _quantize([(x, noise, r, c)], fmt, which, stream)
+    r, c = _rounded(x, fmt, which != "cols", which != "rows", noise)
     return (r, c) if which == "both" else r if c is None else c
 
 
 def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values t stands for (bf16 and fp32 hold them exactly within their range)."""
     _mx("t", t)
-    out = torch.empty(t.shape, dtype=dtype, device=t.device)
     code = _dtype("out", dtype)
-    with _on(out) as stream:
-        L.check(L.lib().psgdk_mx_dequantize(_ptr(t.codes), _ptr(t.scales), *t.shape, _FMT[t.fmt], _ptr(out), code, stream), "mx_dequantize")
+    out = torch.empty(t.shape, dtype=dtype, device=t.device)
+    _launch("mx_dequantize", out.device, L.lib().psgdk_mx_dequantize, t.codes.data_ptr(), t.scales.data_ptr(), *t.shape, _FMT[t.fmt], out.data_ptr(), code)
     return out
 
 
 # ---------------------------------------------------------------------------------------------------------------------------- products
 
-def mx_matmul(a: MxTensor, b: MxTensor, *, out_dtype: torch.dtype = torch.bfloat16, fast_sums: bool = False) -> torch.Tensor:
+def mx_matmul(a: MxTensor, b: MxTensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """A B^T (M x N) of a (M x K) and b (N x K), either in either format; fp32 sums, rounded once to out_dtype.  The same inputs give the same bits:
     a long contraction with few outputs is split, and the parts are added in a fixed order.
     With an fp8 operand the scaled matrix instruction drops the bits of a product below 2^-13 of the largest one it adds (about 2e-5 of a result):
-    that is taken for 16-bit outputs, whose own rounding is a hundred times larger, and for fp32 outputs with fast_sums=True; an fp32 output has
-    fp32 sums throughout otherwise, at half the rate (elements below 2^-126 count as zero there)."""
+    that is taken for 16-bit outputs, whose own rounding is a hundred times larger.  An fp32 output has fp32 sums throughout, at half the rate
+    (elements below 2^-126 count as zero there)."""
     _mx("a", a)
-    _mx("b", b, a.device)
+    _mx("b", b, a.codes.device)
     if a.shape[1] != b.shape[1]:
         raise _bad(f"mx_matmul: a is {a.shape[0]} x {a.shape[1]}, b is {b.shape[0]} x {b.shape[1]}: both are contracted along their rows")
-    code = _dtype("out", out_dtype)
+    return _matmul(a, b, out_dtype, _dtype("out", out_dtype))
+
+
+def _matmul(a, b, out_dtype, code):
     (m, k), n = a.shape, b.shape[0]
-    out = torch.empty((m, n), dtype=out_dtype, device=a.device)
-    lib = L.lib()
-    wb = C.c_size_t()
-    L.check(lib.psgdk_mx_matmul_work_bytes(m, n, k, C.byref(wb)), "mx_matmul_work_bytes")
-    work = torch.empty(wb.value, dtype=torch.uint8, device=a.device) if wb.value else None
-    with _on(out) as stream:
-        L.check(lib.psgdk_mx_matmul(_ptr(a.codes), _ptr(a.scales), m, _FMT[a.fmt], _ptr(b.codes), _ptr(b.scales), n, _FMT[b.fmt], k, _ptr(out), code,
-                                    int(bool(fast_sums)), _ptr(work), wb.value, stream), "mx_matmul")
+    device = a.codes.device
+    out = torch.empty((m, n), dtype=out_dtype, device=device)
+    wb = _work_bytes("psgdk_mx_matmul_work_bytes", m, n, k, _FMT[a.fmt], _FMT[b.fmt], code)
+    work = torch.empty(wb, dtype=torch.uint8, device=device) if wb else None
+    _launch("mx_matmul", device, L.lib().psgdk_mx_matmul, a.codes.data_ptr(), a.scales.data_ptr(), m, _FMT[a.fmt], b.codes.data_ptr(), b.scales.data_ptr(), n,
+            _FMT[b.fmt], k, out.data_ptr(), code, work.data_ptr() if wb else None, wb)
     return out
 
 
@@ -242,26 +266,33 @@ def rms_norm_mx(x: torch.Tensor, gain: torch.Tensor, residual: Optional[torch.Te
     _norm_args(x, gain, residual)
     if torch.is_grad_enabled() and (x.requires_grad or gain.requires_grad or residual is not None and residual.requires_grad):
         raise _bad("rms_norm_mx does not record gradients: use mx_norm_linear, or call it under torch.no_grad()")
-    bits = _fmt(fmt)
+    _fmt(fmt)
     if which not in ("rows", "cols", "both"):
         raise _bad(f'which={which!r}: "rows", "cols" or "both"')
     if not 0.0 <= eps < float("inf"):
         raise _bad(f"eps={eps}")
-    shape = x.shape
-    d = shape[-1]
-    x2, res = x.contiguous(), None if residual is None else residual.contiguous()
-    s = x2 if res is None else torch.empty_like(x2)
-    n = x2.numel() // d
-    inv = torch.empty(n, dtype=torch.float32, device=x.device)
-    r = MxTensor.empty(n, d, fmt, x.device) if which != "cols" else None
-    c = MxTensor.empty(d, n, fmt, x.device) if which != "rows" else None
-    gain = gain.contiguous()
-    with _on(x2) as stream:
-        L.check(L.lib().psgdk_rms_norm_mx(_ptr(x2), _ptr(res), _ptr(gain), _DTYPE[gain.dtype], n, d, _DTYPE[x.dtype], float(eps), bits,
-                                          _ptr(s), _ptr(inv), r and _ptr(r.codes), r and _ptr(r.scales), c and _ptr(c.codes), c and _ptr(c.scales),
-                                          stream), "rms_norm_mx")
-    y = (r, c) if which == "both" else r if c is None else c
-    return y, s, inv
+    r, c, s, inv = _norm(x, gain, residual, eps, fmt, which != "cols", which != "rows")
+    return (r, c) if which == "both" else r if c is None else c, s, inv
+
+
+def _norm(x, gain, residual, eps, fmt, rows, cols):
+    """(y or None, y transposed or None, s, inv) of checked arguments."""
+    d = x.shape[-1]
+    x, gain = x.contiguous(), gain.contiguous()
+    n = x.numel() // d
+    device = x.device
+    if residual is None:
+        s, res = x, None
+    else:
+        residual = residual.contiguous()
+        s, res = torch.empty_like(x), residual.data_ptr()
+    inv = torch.empty(n, dtype=torch.float32, device=device)
+    r = MxTensor.empty(n, d, fmt, device) if rows else None
+    c = MxTensor.empty(d, n, fmt, device) if cols else None
+    _launch("rms_norm_mx", device, L.lib().psgdk_rms_norm_mx, x.data_ptr(), res, gain.data_ptr(), _DTYPE[gain.dtype], n, d, _DTYPE[x.dtype], eps, _FMT[fmt],
+            s.data_ptr(), inv.data_ptr(), r.codes.data_ptr() if rows else None, r.scales.data_ptr() if rows else None,
+            c.codes.data_ptr() if cols else None, c.scales.data_ptr() if cols else None)
+    return r, c, s, inv
 
 
 def rms_norm_mx_backward(dy: torch.Tensor, s: torch.Tensor, gain: torch.Tensor, inv: torch.Tensor, *, ds: Optional[torch.Tensor] = None):
@@ -277,17 +308,22 @@ def rms_norm_mx_backward(dy: torch.Tensor, s: torch.Tensor, gain: torch.Tensor, 
     n = s.numel() // d
     if inv.dtype != torch.float32 or inv.numel() != n:
         raise _bad(f"inv: {n} values in float32, got {inv.dtype} {tuple(inv.shape)}")
+    return _norm_backward(dy, s, gain, inv, ds)
+
+
+def _norm_backward(dy, s, gain, inv, ds):
     dy, s, gain, inv = dy.contiguous(), s.contiguous(), gain.contiguous(), inv.contiguous()
-    ds = None if ds is None else ds.contiguous()
+    if ds is not None:
+        ds = ds.contiguous()
+    d = s.shape[-1]
+    n = s.numel() // d
+    device = s.device
     dx = torch.empty_like(s)
-    dgain = torch.empty(d, dtype=torch.float32, device=s.device)
-    lib = L.lib()
-    wb = C.c_size_t()
-    L.check(lib.psgdk_rms_norm_mx_backward_work_bytes(n, d, C.byref(wb)), "rms_norm_mx_backward_work_bytes")
-    work = torch.empty(max(wb.value, 4), dtype=torch.uint8, device=s.device)
-    with _on(s) as stream:
-        L.check(lib.psgdk_rms_norm_mx_backward(_ptr(dy), _DTYPE[dy.dtype], _ptr(s), _ptr(gain), _DTYPE[gain.dtype], _ptr(inv), _ptr(ds), n, d,
-                                               _DTYPE[s.dtype], _ptr(dx), _ptr(dgain), _ptr(work), wb.value, stream), "rms_norm_mx_backward")
+    dgain = torch.empty(d, dtype=torch.float32, device=device)
+    wb = _work_bytes("psgdk_rms_norm_mx_backward_work_bytes", n, d)
+    work = torch.empty(max(wb, 4), dtype=torch.uint8, device=device)
+    _launch("rms_norm_mx_backward", device, L.lib().psgdk_rms_norm_mx_backward, dy.data_ptr(), _DTYPE[dy.dtype], s.data_ptr(), gain.data_ptr(), _DTYPE[gain.dtype],
+            inv.data_ptr(), None if ds is None else ds.data_ptr(), n, d, _DTYPE[s.dtype], dx.data_ptr(), dgain.data_ptr(), work.data_ptr(), wb)
     return dx, dgain
 
 
@@ -340,15 +376,14 @@ def refresh_mx_weights(weights: Sequence[MxWeight]) -> None:
             raise _bad(f"the parameter is {tuple(p.shape)} now, its MxWeight {w.rows.shape}")
         groups.setdefault((p.device, p.dtype, w.fmt, w.cols is not None), []).append((_rows("param", p), None, w.rows, w.cols))
     for (device, _, fmt, both), items in groups.items():
-        with _on(items[0][0]) as stream:
-            _quantize(items, fmt, "both" if both else "rows", stream)
+        _quantize(items, fmt, device)
         for _, _, r, c in items:
             torch.autograd.graph.increment_version([t for q in (r, c) if q is not None for t in (q.codes, q.scales)])
 
 
 def _restore(ctx, i, shape, fmt) -> MxTensor:
     codes, scales = ctx.saved_tensors[i:i + 2]
-    return MxTensor(codes, scales, shape, fmt)
+    return MxTensor._of(codes, scales, shape, fmt)
 
 
 def _weight_args(x, weight, fmt, grad_fmt):
@@ -376,11 +411,9 @@ def _product_grads(ctx, dout, need_x, need_w, cols_at, act_at, x_dtype):
     """(gradient of the product's input in x_dtype, of the weight) from dout."""
     n, k = ctx.weight_shape
     d2 = _rows("gradient", dout)
-    which = "both" if need_x and need_w else "rows" if need_x else "cols"
-    q = mx_quantize(d2, ctx.grad_fmt, which=which)
-    dr, dc = q if which == "both" else (q, None) if need_x else (None, q)
-    dx = mx_matmul(dr, _restore(ctx, cols_at, (k, n), ctx.weight_fmt), out_dtype=x_dtype, fast_sums=True) if need_x else None
-    dw = mx_matmul(dc, _restore(ctx, act_at, (k, d2.shape[0]), ctx.fmt), out_dtype=ctx.weight_dtype, fast_sums=True) if need_w else None
+    dr, dc = _rounded(d2, ctx.grad_fmt, need_x, need_w)
+    dx = _matmul(dr, _restore(ctx, cols_at, (k, n), ctx.weight_fmt), x_dtype, _DTYPE[x_dtype]) if need_x else None
+    dw = _matmul(dc, _restore(ctx, act_at, (k, d2.shape[0]), ctx.fmt), ctx.weight_dtype, _DTYPE[ctx.weight_dtype]) if need_w else None
     return dx, dw
 
 
@@ -388,9 +421,8 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, param, weight, fmt, grad_fmt):
         need_x, need_w = ctx.needs_input_grad[:2]
-        xr = mx_quantize(x, fmt, which="both" if need_w else "rows")
-        xr, xc = xr if need_w else (xr, None)
-        out = mx_matmul(xr, weight.rows, out_dtype=x.dtype, fast_sums=True)
+        xr, xc = _rounded(_rows("x", x), fmt, True, need_w)
+        out = _matmul(xr, weight.rows, x.dtype, _DTYPE[x.dtype])
         saved = []
         if need_x:
             _need_cols(weight)
@@ -400,7 +432,7 @@ class _Linear(torch.autograd.Function):
         ctx.save_for_backward(*saved)
         ctx.weight_shape, ctx.weight_fmt, ctx.weight_dtype, ctx.fmt, ctx.grad_fmt = weight.rows.shape, weight.fmt, param.dtype, fmt, grad_fmt
         ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
-        return out.view(*x.shape[:-1], weight.rows.shape[0])
+        return out if x.dim() == 2 else out.view(*x.shape[:-1], weight.rows.shape[0])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -415,9 +447,8 @@ class _NormLinear(torch.autograd.Function):
     def forward(ctx, x, residual, gain, param, weight, eps, fmt, grad_fmt):
         need_s = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         need_g, need_w = ctx.needs_input_grad[2:4]
-        y, s, inv = rms_norm_mx(x, gain, residual, eps=eps, fmt=fmt, which="both" if need_w else "rows")
-        yr, yc = y if need_w else (y, None)
-        out = mx_matmul(yr, weight.rows, out_dtype=x.dtype, fast_sums=True)
+        yr, yc, s, inv = _norm(x, gain, residual, eps, fmt, True, need_w)
+        out = _matmul(yr, weight.rows, x.dtype, _DTYPE[x.dtype])
         saved = [s, inv, gain]
         if need_s or need_g:
             _need_cols(weight)
@@ -427,7 +458,7 @@ class _NormLinear(torch.autograd.Function):
         ctx.save_for_backward(*saved)
         ctx.weight_shape, ctx.weight_fmt, ctx.weight_dtype, ctx.fmt, ctx.grad_fmt = weight.rows.shape, weight.fmt, param.dtype, fmt, grad_fmt
         ctx.set_materialize_grads(False)
-        out = out.view(*x.shape[:-1], weight.rows.shape[0])
+        out = out if x.dim() == 2 else out.view(*x.shape[:-1], weight.rows.shape[0])
         return out if residual is None else (out, s)
 
     @staticmethod
@@ -442,7 +473,7 @@ class _NormLinear(torch.autograd.Function):
             # (the gradient of y stays in fp32 between the two kernels: one rounding, at dx)
             dy, dw = _product_grads(ctx, dout, need_y, need_w, 3, 5 if need_y else 3, torch.float32)
             if need_y:
-                dx, dg = rms_norm_mx_backward(dy.view(s.shape), s, gain, inv, ds=ds)
+                dx, dg = _norm_backward(dy.view(s.shape), s, gain, inv, ds)
                 dg = dg.to(gain.dtype)
         elif need_s:
             dx = ds
@@ -452,8 +483,7 @@ class _NormLinear(torch.autograd.Function):
 
 def mx_linear(x: torch.Tensor, weight: MxWeight, *, fmt: str = "fp8", grad_fmt: str = "fp8") -> torch.Tensor:
     """x W^T in x's dtype: x is rounded to `fmt`, W is the weight's kept form.  Backward: dx = MX(dY) W and dW = MX(dY^T) MX(x^T)^T with dY rounded to
-    `grad_fmt` along the contracted axis of each (roundings count as the identity); dW has the parameter's dtype.  The products take
-    mx_matmul's fast_sums: their operands are rounded to 4 significant bits at best."""
+    `grad_fmt` along the contracted axis of each (roundings count as the identity); dW has the parameter's dtype."""
     _weight_args(x, weight, fmt, grad_fmt)
     x, param = _tracked(x, weight.param)
     return _Linear.apply(x, param, weight, fmt, grad_fmt)
@@ -466,5 +496,7 @@ def mx_norm_linear(x: torch.Tensor, gain: torch.Tensor, weight: MxWeight, residu
     _weight_args(x, weight, fmt, grad_fmt)
     _norm_args(x, gain, residual)
     x, residual, gain, param = _tracked(x, residual, gain, weight.param)
+    if not 0.0 <= eps < float("inf"):
+        raise _bad(f"eps={eps}")
     out = _NormLinear.apply(x, residual, gain, param, weight, eps, fmt, grad_fmt)
     return (out, x) if residual is None else out

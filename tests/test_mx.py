@@ -64,7 +64,7 @@ def test_dequantize_refuses(lib):
 
 
 def test_matmul_refuses(lib):
-    ok = [4096, 4096, 70, 4, 4096, 4096, 40, 8, 512, 8192, 0, 0, 65536, 1 << 30, None]
+    ok = [4096, 4096, 70, 4, 4096, 4096, 40, 8, 512, 8192, 0, 65536, 1 << 30, None]
     bad = [(2, -1), (6, -1), (8, -1), (3, 5), (7, 5), (10, 3), (9, None), (0, None), (1, None), (4, None), (5, None), (0, 4104), (4, 4104), (1, 4100), (5, 4100), (9, 8193),
            (2, 1 << 31), (6, 1 << 31), (8, 1 << 31)]
     for i, v in bad:
@@ -72,13 +72,17 @@ def test_matmul_refuses(lib):
         a[i] = v
         assert lib.psgdk_mx_matmul(*a) == 1, (i, v)
     wb = C.c_size_t()
-    assert lib.psgdk_mx_matmul_work_bytes(128, 128, 1 << 16, C.byref(wb)) == 0 and wb.value > 0
-    split = [4096, 4096, 128, 4, 4096, 4096, 128, 8, 1 << 16, 8192, 0, 0, None, 0, None]
+    assert lib.psgdk_mx_matmul_work_bytes(128, 128, 1 << 16, 4, 8, 0, C.byref(wb)) == 0 and wb.value > 0
+    split = [4096, 4096, 128, 4, 4096, 4096, 128, 8, 1 << 16, 8192, 0, None, 0, None]
     assert lib.psgdk_mx_matmul(*split) == 1                                         # split sums without a workspace
-    split[12], split[13] = 65536, wb.value - 1
+    split[11], split[12] = 65536, wb.value - 1
     assert lib.psgdk_mx_matmul(*split) == 1
-    assert lib.psgdk_mx_matmul_work_bytes(1, 1, -1, C.byref(wb)) == 1 and lib.psgdk_mx_matmul_work_bytes(1, 1, 1, None) == 1
-    assert lib.psgdk_mx_matmul(None, None, 0, 4, None, None, 40, 4, 64, None, 0, 0, None, 0, None) == 0
+    assert lib.psgdk_mx_matmul_work_bytes(1, 1, -1, 4, 4, 0, C.byref(wb)) == 1 and lib.psgdk_mx_matmul_work_bytes(1, 1, 1, 4, 4, 0, None) == 1
+    for i, v in ((6, (1 << 22) + 1), (8, (1 << 23) + 1)):
+        a = list(ok)
+        a[i] = v
+        assert lib.psgdk_mx_matmul(*a) == 2, (i, v)
+    assert lib.psgdk_mx_matmul(None, None, 0, 4, None, None, 40, 4, 64, None, 0, None, 0, None) == 0
 
 
 def test_norm_refuses(lib):
