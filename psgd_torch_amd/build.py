@@ -33,9 +33,7 @@ def needs_build() -> bool:
 
 # (packed fp32 off in the MX unit: some forms of the packed instructions hipcc makes from plain float code have returned wrong results)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result"]
-# (accumulators in the VGPR form: left to itself the compiler moves the 256 accumulators of the large tile between both halves of the register file
-# and spills; with it the main loop has no scratch access)
-MX_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+MX_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _run(cmds, verbose):

@@ -94,7 +94,7 @@ static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, bool wide) {
         return p;
     }
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    p.bm = p.bn = big >= 256 && !wide ? 256 : 128;
+    p.bm = p.bn = big >= 256 ? 256 : 128;
     const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
     while (p.splits < 16 && tiles * p.splits * 2 <= 512 && KS / (p.splits * 2) >= 2) p.splits *= 2;
     return p;
@@ -109,8 +109,8 @@ static int mx_launch_product(const MxGemm& g, const MxPlan& p, hipStream_t st) {
 #undef MX_SKINNY
     } else {
         const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
-        if constexpr (!WIDE) if (p.bm == 256) mx_tile_gemm_kernel<FA, FB, WIDE, 256, 256><<<grid, 256, 0, st>>>(g);
-        if (p.bm == 128) mx_tile_gemm_kernel<FA, FB, WIDE, 128, 128><<<grid, 256, 0, st>>>(g);
+        if (p.bm == 256) mx_tile_gemm_kernel<FA, FB, WIDE, 256, 256, 2><<<grid, 256, 0, st>>>(g);
+        else mx_tile_gemm_kernel<FA, FB, WIDE, 128, 128, 2><<<grid, 256, 0, st>>>(g);
     }
     MX_LAUNCHED();
     if (g.part) {
