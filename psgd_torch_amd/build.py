@@ -9,8 +9,8 @@ import sys
 import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-# two translation units, compiled side by side: the preconditioner engine, and the microscaled (MX) operators
-SRCS = [os.path.join(HERE, "csrc", "psgdk.hip"), os.path.join(HERE, "csrc", "psgdk_mx.hip")]
+# translation units, compiled side by side: the preconditioner engine, the microscaled (MX) operators, their products
+SRCS = [os.path.join(HERE, "csrc", f) for f in ("psgdk.hip", "psgdk_mx.hip", "psgdk_mx_gemm.hip")]
 OUT = os.path.join(HERE, "libpsgdk.so")
 # the measurement probes (matrix-core / HBM ceilings of the chip for bench.py's peak_measured) are a library of their own:
 # the product library carries no probe kernels
@@ -31,7 +31,7 @@ def needs_build() -> bool:
     return any(os.path.getmtime(s) > t for s in _sources())
 
 
-# (packed fp32 off in the MX unit: some forms of the packed instructions hipcc makes from plain float code have returned wrong results)
+# (packed fp32 off in the MX units: some forms of the packed instructions hipcc makes from plain float code have returned wrong results)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result"]
 MX_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
@@ -55,7 +55,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     with tempfile.TemporaryDirectory() as tmp:
         objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in SRCS]
-        _run([[hipcc, *FLAGS, *(MX_FLAGS if s.endswith("_mx.hip") else []), "-c", s, "-o", o] for s, o in zip(SRCS, objs)]
+        _run([[hipcc, *FLAGS, *(MX_FLAGS if "_mx" in os.path.basename(s) else []), "-c", s, "-o", o] for s, o in zip(SRCS, objs)]
              + [[hipcc, *FLAGS, "-shared", PROBE_SRC, "-o", PROBE_OUT]], verbose)
         _run([[hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", OUT]], verbose)
     return OUT

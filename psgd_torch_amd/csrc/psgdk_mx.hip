@@ -1,27 +1,7 @@
-// psgdk_mx.hip -- the C ABI of the microscaled (MX) operators (include/psgdk.h, "microscaled numbers"): argument checks, choice of kernel, launches.
-// A translation unit of its own: nothing here shares state with a plan; every call is stream-ordered and keeps nothing.
-#include <cstring>
-#include "../../include/psgdk.h"
-#include "gemm_mx.hiph"
-
-extern "C" int psgdk_note_hip_error(int e);      // psgdk.hip: what psgdk_last_hip_error returns
-
-#define MX_HIPCHK(expr)                                                   \
-    do {                                                                  \
-        const hipError_t _e = (expr);                                     \
-        if (_e != hipSuccess) return psgdk_note_hip_error((int)_e);       \
-    } while (0)
-#define MX_LAUNCHED() MX_HIPCHK(hipGetLastError())
-
-static const int64_t kMaxDim = (1ll << 31) - 65536;      // rows and columns are 32-bit in the kernels; offsets are 64-bit
-static const int64_t kMaxN = 1ll << 22;                  // a product's columns: 256 rows of the output lie within 32-bit offsets
-static const int64_t kMaxK = 1ll << 23;                  // a product's contraction: 256 stored rows of an operand tile lie within 32-bit offsets
-
-static bool mx_fmt_ok(int f) { return f == PSGDK_MX_FP4 || f == PSGDK_MX_FP8; }
-static bool mx_dtype_ok(int d) { return d == PSGDK_BF16 || d == PSGDK_F32 || d == PSGDK_F16; }
-static int mx_size(int d) { return d == PSGDK_F32 ? 4 : 2; }
-static bool mx_aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-static int64_t mx_pad(int64_t n) { return (n + MX_PAD - 1) / MX_PAD * MX_PAD; }
+// psgdk_mx.hip -- the C ABI of the microscaled (MX) operators but the product (include/psgdk.h, "microscaled numbers"): argument checks, choice of
+// kernel, launches.  Nothing here shares state with a plan; every call is stream-ordered and keeps nothing.
+#include <type_traits>
+#include "mx_host.hiph"
 
 // calls f with a null pointer of the element type
 template <typename F>
@@ -29,96 +9,51 @@ static int mx_by_dtype(int d, F&& f) {
     return d == PSGDK_BF16 ? f((bf16_t*)nullptr) : d == PSGDK_F32 ? f((float*)nullptr) : f((mx_half*)nullptr);
 }
 
-template <typename T, int FMT, bool NOISE, bool VEC>
+template <typename T, int FMT, bool NOISE>
 static int mx_launch_round(const MxJobs& a, unsigned grid, bool rows, bool cols, hipStream_t st) {
-    if (!cols) mx_rows_kernel<T, FMT, NOISE, VEC><<<grid, 256, 0, st>>>(a);
-    else if (rows) mx_tile_kernel<T, FMT, true, NOISE, false, VEC><<<grid, 256, 0, st>>>(a, MxNormArgs{nullptr, nullptr, 0});
-    else mx_tile_kernel<T, FMT, false, NOISE, false, VEC><<<grid, 256, 0, st>>>(a, MxNormArgs{nullptr, nullptr, 0});
+    if (!cols) mx_rows_kernel<T, FMT, NOISE><<<grid, 256, 0, st>>>(a);
+    else if (rows) mx_tile_kernel<T, FMT, true, NOISE, false><<<grid, 256, 0, st>>>(a, MxNormArgs{nullptr, nullptr, 0});
+    else mx_tile_kernel<T, FMT, false, NOISE, false><<<grid, 256, 0, st>>>(a, MxNormArgs{nullptr, nullptr, 0});
     MX_LAUNCHED();
     return PSGDK_OK;
 }
-template <typename T, int FMT, bool NOISE>
-static int mx_launch_round(const MxJobs& a, unsigned grid, bool rows, bool cols, bool vec, hipStream_t st) {
-    return vec ? mx_launch_round<T, FMT, NOISE, true>(a, grid, rows, cols, st) : mx_launch_round<T, FMT, NOISE, false>(a, grid, rows, cols, st);
-}
 
-template <typename T, int FMT, int THREADS, int CH, bool VEC>
+template <typename T, int FMT, int THREADS, int CH>
 static void mx_norm_one(const void* x, const void* res, const void* gain, int gdt, void* s, float* inv, uint8_t* codes, uint8_t* scales, int rows,
                         int cols, float eps, hipStream_t st) {
     const unsigned grid = THREADS == 64 ? (rows + 3) / 4 : rows;
-    rms_norm_mx_kernel<T, FMT, THREADS, CH, VEC><<<grid, 256, 0, st>>>((const T*)x, (const T*)res, gain, gdt, (T*)s, inv, codes, scales, rows, cols, eps);
+    rms_norm_mx_kernel<T, FMT, THREADS, CH><<<grid, 256, 0, st>>>((const T*)x, (const T*)res, gain, gdt, (T*)s, inv, codes, scales, rows, cols, eps);
 }
 // one wave a row up to 2048 columns, a workgroup a row up to 16384
-template <typename T, int FMT, bool VEC, typename... A>
+template <typename T, int FMT, typename... A>
 static void mx_norm_by_cols(int cols, A... a) {
-    if (cols <= 512) mx_norm_one<T, FMT, 64, 1, VEC>(a...);
-    else if (cols <= 1024) mx_norm_one<T, FMT, 64, 2, VEC>(a...);
-    else if (cols <= 2048) mx_norm_one<T, FMT, 64, 4, VEC>(a...);
-    else if (cols <= 4096) mx_norm_one<T, FMT, 256, 2, VEC>(a...);
-    else if (cols <= 8192) mx_norm_one<T, FMT, 256, 4, VEC>(a...);
-    else mx_norm_one<T, FMT, 256, 8, VEC>(a...);
+    if (cols <= 512) mx_norm_one<T, FMT, 64, 1>(a...);
+    else if (cols <= 1024) mx_norm_one<T, FMT, 64, 2>(a...);
+    else if (cols <= 2048) mx_norm_one<T, FMT, 64, 4>(a...);
+    else if (cols <= 4096) mx_norm_one<T, FMT, 256, 2>(a...);
+    else if (cols <= 8192) mx_norm_one<T, FMT, 256, 4>(a...);
+    else mx_norm_one<T, FMT, 256, 8>(a...);
 }
 
-template <typename T, typename TD, int THREADS, int CH, bool VEC>
+template <typename T, typename TD, int THREADS, int CH>
 static void mx_norm_back_one(unsigned grid, const void* dy, const void* s, const void* gain, int gdt, const float* inv, const void* ds, void* dx,
                              float* part, int rows, int cols, hipStream_t st) {
-    rms_norm_mx_backward_kernel<T, TD, THREADS, CH, VEC>
+    rms_norm_mx_backward_kernel<T, TD, THREADS, CH>
         <<<grid, 256, 0, st>>>((const TD*)dy, (const T*)s, gain, gdt, inv, (const T*)ds, (T*)dx, part, rows, cols);
 }
-template <typename T, typename TD, bool VEC, typename... A>
+template <typename T, typename TD, typename... A>
 static void mx_norm_back_by_cols(int cols, A... a) {
-    if (cols <= 512) mx_norm_back_one<T, TD, 64, 1, VEC>(a...);
-    else if (cols <= 1024) mx_norm_back_one<T, TD, 64, 2, VEC>(a...);
-    else if (cols <= 2048) mx_norm_back_one<T, TD, 64, 4, VEC>(a...);
-    else if (cols <= 4096) mx_norm_back_one<T, TD, 256, 2, VEC>(a...);
-    else if (cols <= 8192) mx_norm_back_one<T, TD, 256, 4, VEC>(a...);
-    else mx_norm_back_one<T, TD, 256, 8, VEC>(a...);
+    if (cols <= 512) mx_norm_back_one<T, TD, 64, 1>(a...);
+    else if (cols <= 1024) mx_norm_back_one<T, TD, 64, 2>(a...);
+    else if (cols <= 2048) mx_norm_back_one<T, TD, 64, 4>(a...);
+    else if (cols <= 4096) mx_norm_back_one<T, TD, 256, 2>(a...);
+    else if (cols <= 8192) mx_norm_back_one<T, TD, 256, 4>(a...);
+    else mx_norm_back_one<T, TD, 256, 8>(a...);
 }
 // lines of the gain gradient's shares: enough workgroups to fill the chip, no more (every line costs 8 bytes a column)
 static int mx_back_lines(int64_t rows, int64_t cols) {
     const int64_t per = cols <= 2048 ? 4 : 1, want = (rows + per - 1) / per;
     return (int)(want < 512 ? want : 512);
-}
-
-// ---- products ----------------------------------------------------------------------------------------------------------------------------
-// a 32-bit output with an 8-bit operand: fp32 sums through bf16 products (gemm_mx.hiph)
-static bool mx_wide(int a_fmt, int b_fmt, int out_dtype) { return out_dtype == PSGDK_F32 && (a_fmt == PSGDK_MX_FP8 || b_fmt == PSGDK_MX_FP8); }
-struct MxPlan { bool skinny; int mt, nt, bm, bn, splits; };
-static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, bool wide) {
-    MxPlan p{};
-    p.splits = 1;
-    if (M <= 64) {
-        p.skinny = true;
-        p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-        p.nt = N >= 16 * 2 * 512 ? 2 : 1;
-        return p;
-    }
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    p.bm = p.bn = big >= 256 ? 256 : 128;
-    const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
-    while (p.splits < 16 && tiles * p.splits * 2 <= 512 && KS / (p.splits * 2) >= 2) p.splits *= 2;
-    return p;
-}
-
-template <int FA, int FB, bool WIDE>
-static int mx_launch_product(const MxGemm& g, const MxPlan& p, hipStream_t st) {
-    if (p.skinny) {
-        const unsigned grid = (unsigned)((g.N + 16 * p.nt - 1) / (16 * p.nt));
-#define MX_SKINNY(MT, NT) if (p.mt == MT && p.nt == NT) mx_skinny_kernel<FA, FB, WIDE, MT, NT><<<grid, 512, 0, st>>>(g);
-        MX_SKINNY(1, 1) MX_SKINNY(2, 1) MX_SKINNY(4, 1) MX_SKINNY(1, 2) MX_SKINNY(2, 2) MX_SKINNY(4, 2)
-#undef MX_SKINNY
-    } else {
-        const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
-        if (p.bm == 256) mx_tile_gemm_kernel<FA, FB, WIDE, 256, 256, 2><<<grid, 256, 0, st>>>(g);
-        else mx_tile_gemm_kernel<FA, FB, WIDE, 128, 128, 2><<<grid, 256, 0, st>>>(g);
-    }
-    MX_LAUNCHED();
-    if (g.part) {
-        const int64_t total = (int64_t)g.M * g.N;
-        mx_join_kernel<<<(unsigned)((total + 1023) / 1024), 256, 0, st>>>(g.part, g.out, g.out_dtype, g.splits, total);
-        MX_LAUNCHED();
-    }
-    return PSGDK_OK;
 }
 
 extern "C" {
@@ -153,7 +88,6 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
         MxJobs a;
         a.n = 0;
         int64_t wgs = 0;
-        bool vec = true;
         for (; i < count && a.n < MX_JOBS; ++i) {
             const psgdk_mx_tensor& q = t[i];
             if (q.rows == 0 || q.cols == 0) continue;
@@ -165,14 +99,13 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
             MxJob& j = a.j[a.n++];
             j = MxJob{q.x, (const uint8_t*)q.noise, (uint8_t*)q.codes, (uint8_t*)q.scales, (uint8_t*)q.codes_t, (uint8_t*)q.scales_t, q.ld, (int)q.rows,
                       (int)q.cols, (unsigned)wgs, FastDiv::make((unsigned)(cols ? tiles_n : units))};
-            vec = vec && mx_aligned(q.x, 16) && q.ld * mx_size(dtype) % 16 == 0;
             wgs += need;
         }
         if (a.n == 0) continue;
         const int rc = mx_by_dtype(dtype, [&](auto* e) {
             using T = std::remove_pointer_t<decltype(e)>;
-            if (fmt == PSGDK_MX_FP8) return mx_launch_round<T, 8, false>(a, (unsigned)wgs, rows, cols, vec, st);
-            return noise ? mx_launch_round<T, 4, true>(a, (unsigned)wgs, rows, cols, vec, st) : mx_launch_round<T, 4, false>(a, (unsigned)wgs, rows, cols, vec, st);
+            if (fmt == PSGDK_MX_FP8) return mx_launch_round<T, 8, false>(a, (unsigned)wgs, rows, cols, st);
+            return noise ? mx_launch_round<T, 4, true>(a, (unsigned)wgs, rows, cols, st) : mx_launch_round<T, 4, false>(a, (unsigned)wgs, rows, cols, st);
         });
         if (rc != PSGDK_OK) return rc;
     }
@@ -185,54 +118,17 @@ int psgdk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int
     if (!codes || !scales || !out || !mx_aligned(codes, 16) || !mx_aligned(out, mx_size(out_dtype))) return PSGDK_ERR_INVALID;
     const int64_t units = mx_pad(cols) / MX_PAD, need = (rows * units + 7) / 8;
     if (need > (1ll << 28)) return PSGDK_ERR_UNSUPPORTED;
-    const bool vec = mx_aligned(out, 16) && cols * mx_size(out_dtype) % 16 == 0;
     const FastDiv div = FastDiv::make((unsigned)units);
     const hipStream_t st = (hipStream_t)stream;
     return mx_by_dtype(out_dtype, [&](auto* e) {
         using T = std::remove_pointer_t<decltype(e)>;
-#define MX_DEQ(F, V) mx_dequantize_kernel<T, F, V><<<(unsigned)need, 256, 0, st>>>((const uint8_t*)codes, (const uint8_t*)scales, (T*)out, (int)rows, (int)cols, div)
-        if (fmt == PSGDK_MX_FP4) { if (vec) MX_DEQ(4, true); else MX_DEQ(4, false); }
-        else { if (vec) MX_DEQ(8, true); else MX_DEQ(8, false); }
+#define MX_DEQ(F) mx_dequantize_kernel<T, F><<<(unsigned)need, 256, 0, st>>>((const uint8_t*)codes, (const uint8_t*)scales, (T*)out, (int)rows, (int)cols, div)
+        if (fmt == PSGDK_MX_FP4) MX_DEQ(4);
+        else MX_DEQ(8);
 #undef MX_DEQ
         MX_LAUNCHED();
         return (int)PSGDK_OK;
     });
-}
-
-int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int out_dtype, size_t* bytes) {
-    if (m < 0 || n < 0 || k < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim || !bytes) return PSGDK_ERR_INVALID;
-    if (!mx_fmt_ok(a_fmt) || !mx_fmt_ok(b_fmt) || !mx_dtype_ok(out_dtype)) return PSGDK_ERR_INVALID;
-    const MxPlan p = mx_plan(m, n, mx_pad(k) / MX_PAD, mx_wide(a_fmt, b_fmt, out_dtype));
-    *bytes = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
-    return PSGDK_OK;
-}
-
-int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_fmt, const void* b_codes, const void* b_scales, int64_t n, int b_fmt,
-                    int64_t k, void* out, int out_dtype, void* work, size_t work_bytes, void* stream) {
-    if (m < 0 || n < 0 || k < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim) return PSGDK_ERR_INVALID;
-    if (!mx_fmt_ok(a_fmt) || !mx_fmt_ok(b_fmt) || !mx_dtype_ok(out_dtype)) return PSGDK_ERR_INVALID;
-    if (k > kMaxK || n > kMaxN) return PSGDK_ERR_UNSUPPORTED;
-    if (m == 0 || n == 0) return PSGDK_OK;
-    if (!out || !mx_aligned(out, mx_size(out_dtype))) return PSGDK_ERR_INVALID;
-    if (k > 0 && (!a_codes || !a_scales || !b_codes || !b_scales)) return PSGDK_ERR_INVALID;
-    if (!mx_aligned(a_codes, 16) || !mx_aligned(b_codes, 16) || !mx_aligned(a_scales, 8) || !mx_aligned(b_scales, 8)) return PSGDK_ERR_INVALID;
-    const int64_t KS = mx_pad(k) / MX_PAD;
-    const bool wide = mx_wide(a_fmt, b_fmt, out_dtype);
-    const MxPlan p = mx_plan(m, n, KS, wide);
-    const size_t need = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
-    if (need && (!work || work_bytes < need || !mx_aligned(work, 16))) return PSGDK_ERR_INVALID;
-    const int64_t tm = p.skinny ? 1 : (m + p.bm - 1) / p.bm, tn = p.skinny ? 1 : (n + p.bn - 1) / p.bn;
-    if (tm * tn * p.splits > (1ll << 28) || (need && m * n / 1024 > (1ll << 28))) return PSGDK_ERR_UNSUPPORTED;
-    const MxGemm g{(const uint8_t*)a_codes, (const uint8_t*)a_scales, (const uint8_t*)b_codes, (const uint8_t*)b_scales, out, need ? (float*)work : nullptr, n,
-                   (int)m, (int)n, (int)KS, out_dtype, p.splits, (int)tm, (int)tn};
-    const hipStream_t st = (hipStream_t)stream;
-    if (a_fmt == PSGDK_MX_FP4 && b_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 4, false>(g, p, st);
-    if (wide) {
-        if (a_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 8, true>(g, p, st);
-        return b_fmt == PSGDK_MX_FP4 ? mx_launch_product<8, 4, true>(g, p, st) : mx_launch_product<8, 8, true>(g, p, st);
-    }
-    if (a_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 8, false>(g, p, st);
-    return b_fmt == PSGDK_MX_FP4 ? mx_launch_product<8, 4, false>(g, p, st) : mx_launch_product<8, 8, false>(g, p, st);
 }
 
 int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int gain_dtype, int64_t rows, int64_t cols, int dtype, float eps, int fmt,
@@ -244,16 +140,15 @@ int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int
     const int size = mx_size(dtype);
     if (!mx_aligned(x, size) || !mx_aligned(residual, size) || !mx_aligned(s, size) || !mx_aligned(gain, mx_size(gain_dtype)) || !mx_aligned(inv, 4) ||
         !mx_aligned(codes, 16) || !mx_aligned(codes_t, 16)) return PSGDK_ERR_INVALID;
-    const bool vec = mx_aligned(x, 16) && mx_aligned(residual, 16) && mx_aligned(residual ? s : nullptr, 16) && cols * size % 16 == 0;
     const hipStream_t st = (hipStream_t)stream;
     const int64_t tiles_n = (cols + 256 / size - 1) / (256 / size), tiles = mx_pad(rows) / 128 * tiles_n;
     if (codes_t && tiles > (1ll << 28)) return PSGDK_ERR_UNSUPPORTED;
     return mx_by_dtype(dtype, [&](auto* e) {
         using T = std::remove_pointer_t<decltype(e)>;
-#define MX_NORM(F, V) mx_norm_by_cols<T, F, V>((int)cols, x, residual, gain, gain_dtype, s, inv, (uint8_t*)codes, (uint8_t*)scales, (int)rows, (int)cols, eps, st)
-        if (!codes) { if (vec) MX_NORM(0, true); else MX_NORM(0, false); }
-        else if (fmt == PSGDK_MX_FP4) { if (vec) MX_NORM(4, true); else MX_NORM(4, false); }
-        else { if (vec) MX_NORM(8, true); else MX_NORM(8, false); }
+#define MX_NORM(F) mx_norm_by_cols<T, F>((int)cols, x, residual, gain, gain_dtype, s, inv, (uint8_t*)codes, (uint8_t*)scales, (int)rows, (int)cols, eps, st)
+        if (!codes) MX_NORM(0);
+        else if (fmt == PSGDK_MX_FP4) MX_NORM(4);
+        else MX_NORM(8);
 #undef MX_NORM
         MX_LAUNCHED();
         if (codes_t) {
@@ -262,9 +157,9 @@ int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int
             a.j[0] = MxJob{residual ? s : x, nullptr, nullptr, nullptr, (uint8_t*)codes_t, (uint8_t*)scales_t, cols, (int)rows, (int)cols, 0u,
                            FastDiv::make((unsigned)tiles_n)};
             const MxNormArgs n{inv, gain, gain_dtype};
-#define MX_NT(F, V) mx_tile_kernel<T, F, false, false, true, V><<<(unsigned)tiles, 256, 0, st>>>(a, n)
-            if (fmt == PSGDK_MX_FP4) { if (vec) MX_NT(4, true); else MX_NT(4, false); }
-            else { if (vec) MX_NT(8, true); else MX_NT(8, false); }
+#define MX_NT(F) mx_tile_kernel<T, F, false, false, true><<<(unsigned)tiles, 256, 0, st>>>(a, n)
+            if (fmt == PSGDK_MX_FP4) MX_NT(4);
+            else MX_NT(8);
 #undef MX_NT
             MX_LAUNCHED();
         }
@@ -291,21 +186,20 @@ int psgdk_rms_norm_mx_backward(const void* dy, int dy_dtype, const void* s, cons
         if (!mx_aligned(dy, mx_size(dy_dtype)) || !mx_aligned(s, size) || !mx_aligned(ds, size) || !mx_aligned(dx, size) || !mx_aligned(inv, 4) ||
             !mx_aligned(gain, mx_size(gain_dtype))) return PSGDK_ERR_INVALID;
     }
-    const bool vec = mx_aligned(dy, 16) && mx_aligned(s, 16) && mx_aligned(ds, 16) && mx_aligned(dx, 16) && cols * size % 16 == 0;
     const hipStream_t st = (hipStream_t)stream;
     if (rows > 0) {
         const int rc = mx_by_dtype(dtype, [&](auto* e) {
             using T = std::remove_pointer_t<decltype(e)>;
-#define MX_BACK(TD, V) mx_norm_back_by_cols<T, TD, V>((int)cols, (unsigned)lines, dy, s, gain, gain_dtype, inv, ds, dx, (float*)work, (int)rows, (int)cols, st)
-            if (dy_dtype == PSGDK_F32) { if (vec) MX_BACK(float, true); else MX_BACK(float, false); }
-            else { if (vec) MX_BACK(T, true); else MX_BACK(T, false); }
+#define MX_BACK(TD) mx_norm_back_by_cols<T, TD>((int)cols, (unsigned)lines, dy, s, gain, gain_dtype, inv, ds, dx, (float*)work, (int)rows, (int)cols, st)
+            if (dy_dtype == PSGDK_F32) MX_BACK(float);
+            else MX_BACK(T);
 #undef MX_BACK
             MX_LAUNCHED();
             return (int)PSGDK_OK;
         });
         if (rc != PSGDK_OK) return rc;
     }
-    rms_norm_mx_dgain_kernel<<<(unsigned)((cols + 63) / 64), 256, 0, st>>>((const float*)work, dgain, rows > 0 ? lines : 0, (int)cols);
+    rms_norm_mx_dgain_kernel<<<(unsigned)((cols + 31) / 32), 1024, 0, st>>>((const float*)work, dgain, rows > 0 ? lines : 0, (int)cols);
     MX_LAUNCHED();
     return PSGDK_OK;
 }

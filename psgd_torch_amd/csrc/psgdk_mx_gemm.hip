@@ -1,0 +1,83 @@
+// psgdk_mx_gemm.hip -- psgdk_mx_matmul (include/psgdk.h, "microscaled numbers"): argument checks, choice of kernel, launches.
+#include "mx_host.hiph"
+#include "gemm_mx.hiph"
+
+// a 32-bit output with an 8-bit operand: fp32 sums through bf16 products (gemm_mx.hiph)
+static bool mx_wide(int a_fmt, int b_fmt, int out_dtype) { return out_dtype == PSGDK_F32 && (a_fmt == PSGDK_MX_FP8 || b_fmt == PSGDK_MX_FP8); }
+struct MxPlan { bool skinny; int mt, nt, bm, bn, splits; };
+static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, bool wide) {
+    MxPlan p{};
+    p.splits = 1;
+    if (M <= 64) {
+        p.skinny = true;
+        p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+        p.nt = N >= 16 * 2 * 512 ? 2 : 1;
+        return p;
+    }
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
+    p.bm = p.bn = big >= 256 && !wide ? 256 : 128;
+    const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
+    while (p.splits < 16 && tiles * p.splits * 2 <= 512 && KS / (p.splits * 2) >= 2) p.splits *= 2;
+    return p;
+}
+
+template <int FA, int FB, bool WIDE>
+static int mx_launch_product(const MxGemm& g, const MxPlan& p, hipStream_t st) {
+    if (p.skinny) {
+        const unsigned grid = (unsigned)((g.N + 16 * p.nt - 1) / (16 * p.nt));
+#define MX_SKINNY(MT, NT) if (p.mt == MT && p.nt == NT) mx_skinny_kernel<FA, FB, WIDE, MT, NT><<<grid, 512, 0, st>>>(g);
+        MX_SKINNY(1, 1) MX_SKINNY(2, 1) MX_SKINNY(4, 1) MX_SKINNY(1, 2) MX_SKINNY(2, 2) MX_SKINNY(4, 2)
+#undef MX_SKINNY
+    } else {
+        const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
+        if constexpr (!WIDE) if (p.bm == 256) mx_tile_gemm_kernel<FA, FB, WIDE, 256, 256, 2><<<grid, 256, 0, st>>>(g);
+        if (p.bm == 128) mx_tile_gemm_kernel<FA, FB, WIDE, 128, 128, 2><<<grid, 256, 0, st>>>(g);
+    }
+    MX_LAUNCHED();
+    if (g.part) {
+        const int64_t total = (int64_t)g.M * g.N;
+        mx_join_kernel<<<(unsigned)((total + 1023) / 1024), 256, 0, st>>>(g.part, g.out, g.out_dtype, g.splits, total);
+        MX_LAUNCHED();
+    }
+    return PSGDK_OK;
+}
+
+extern "C" {
+
+int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int out_dtype, size_t* bytes) {
+    if (m < 0 || n < 0 || k < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim || !bytes) return PSGDK_ERR_INVALID;
+    if (!mx_fmt_ok(a_fmt) || !mx_fmt_ok(b_fmt) || !mx_dtype_ok(out_dtype)) return PSGDK_ERR_INVALID;
+    const MxPlan p = mx_plan(m, n, mx_pad(k) / MX_PAD, mx_wide(a_fmt, b_fmt, out_dtype));
+    *bytes = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
+    return PSGDK_OK;
+}
+
+int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_fmt, const void* b_codes, const void* b_scales, int64_t n, int b_fmt,
+                    int64_t k, void* out, int out_dtype, void* work, size_t work_bytes, void* stream) {
+    if (m < 0 || n < 0 || k < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim) return PSGDK_ERR_INVALID;
+    if (!mx_fmt_ok(a_fmt) || !mx_fmt_ok(b_fmt) || !mx_dtype_ok(out_dtype)) return PSGDK_ERR_INVALID;
+    if (k > kMaxK || n > kMaxN) return PSGDK_ERR_UNSUPPORTED;
+    if (m == 0 || n == 0) return PSGDK_OK;
+    if (!out || !mx_aligned(out, mx_size(out_dtype))) return PSGDK_ERR_INVALID;
+    if (k > 0 && (!a_codes || !a_scales || !b_codes || !b_scales)) return PSGDK_ERR_INVALID;
+    if (!mx_aligned(a_codes, 16) || !mx_aligned(b_codes, 16) || !mx_aligned(a_scales, 8) || !mx_aligned(b_scales, 8)) return PSGDK_ERR_INVALID;
+    const int64_t KS = mx_pad(k) / MX_PAD;
+    const bool wide = mx_wide(a_fmt, b_fmt, out_dtype);
+    const MxPlan p = mx_plan(m, n, KS, wide);
+    const size_t need = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
+    if (need && (!work || work_bytes < need || !mx_aligned(work, 16))) return PSGDK_ERR_INVALID;
+    const int64_t tm = p.skinny ? 1 : (m + p.bm - 1) / p.bm, tn = p.skinny ? 1 : (n + p.bn - 1) / p.bn;
+    if (tm * tn * p.splits > (1ll << 28) || (need && m * n / 1024 > (1ll << 28))) return PSGDK_ERR_UNSUPPORTED;
+    const MxGemm g{(const uint8_t*)a_codes, (const uint8_t*)a_scales, (const uint8_t*)b_codes, (const uint8_t*)b_scales, out, need ? (float*)work : nullptr, n,
+                   (int)m, (int)n, (int)KS, out_dtype, p.splits, (int)tm, (int)tn};
+    const hipStream_t st = (hipStream_t)stream;
+    if (a_fmt == PSGDK_MX_FP4 && b_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 4, false>(g, p, st);
+    if (wide) {
+        if (a_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 8, true>(g, p, st);
+        return b_fmt == PSGDK_MX_FP4 ? mx_launch_product<8, 4, true>(g, p, st) : mx_launch_product<8, 8, true>(g, p, st);
+    }
+    if (a_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 8, false>(g, p, st);
+    return b_fmt == PSGDK_MX_FP4 ? mx_launch_product<8, 4, false>(g, p, st) : mx_launch_product<8, 8, false>(g, p, st);
+}
+
+}  // extern "C"
