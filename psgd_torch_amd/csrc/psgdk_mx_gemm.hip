@@ -4,18 +4,24 @@
 
 // a 32-bit output with an 8-bit operand: fp32 sums through bf16 products (gemm_mx.hiph)
 static bool mx_wide(int a_fmt, int b_fmt, int out_dtype) { return out_dtype == PSGDK_F32 && (a_fmt == PSGDK_MX_FP8 || b_fmt == PSGDK_MX_FP8); }
-struct MxPlan { bool skinny; int mt, nt, bm, bn, splits; };
+struct MxPlan { bool skinny; int mt, kw, bm, bn, splits; };
 static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, bool wide) {
     MxPlan p{};
     p.splits = 1;
-    if (M <= 64) {
+    // Few rows: the kernel without LDS reads A anew for every 16 rows of B, the tiles once for 128.  Measured (fp8 x fp4, us, without / tiles): M = 5:
+    // N = K = 4096 4.8 / 8.8, 8192 13.3 / 13.4; M = 16: 6.0 / 9.4, 17.4 / 13.9, 50257 x 768 10.9 / 8.2; M = 64: 12.8 / 12.7, 42.7 / 18.0; M = 1:
+    // 50257 x 768 6.8 without (A's one row costs nothing).
+    const int64_t mt = (M + 15) / 16;
+    if (M <= 4 || (M <= 64 && mt * N * KS <= (1ll << 25) / 256)) {
         p.skinny = true;
-        p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-        p.nt = N >= 16 * 2 * 512 ? 2 : 1;
+        p.mt = (int)mt;
+        p.kw = 1;                                        // two waves a SIMD or more, none without a share of K
+        while (p.kw < 8 && (N + 15) / 16 * p.kw < 2048 && p.kw < KS) p.kw *= 2;
         return p;
     }
     const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
     p.bm = p.bn = big >= 256 && !wide ? 256 : 128;
+    if (M <= 64) p.bm = 64;
     const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
     while (p.splits < 16 && tiles * p.splits * 2 <= 512 && KS / (p.splits * 2) >= 2) p.splits *= 2;
     return p;
@@ -24,14 +30,17 @@ static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, bool wide) {
 template <int FA, int FB, bool WIDE>
 static int mx_launch_product(const MxGemm& g, const MxPlan& p, hipStream_t st) {
     if (p.skinny) {
-        const unsigned grid = (unsigned)((g.N + 16 * p.nt - 1) / (16 * p.nt));
-#define MX_SKINNY(MT, NT) if (p.mt == MT && p.nt == NT) mx_skinny_kernel<FA, FB, WIDE, MT, NT><<<grid, 512, 0, st>>>(g);
-        MX_SKINNY(1, 1) MX_SKINNY(2, 1) MX_SKINNY(4, 1) MX_SKINNY(1, 2) MX_SKINNY(2, 2) MX_SKINNY(4, 2)
+        const int64_t groups = ((int64_t)g.N + 15) / 16;
+        const int waves = p.kw == 8 ? 8 : 4;
+        const unsigned grid = (unsigned)((groups * p.kw + waves - 1) / waves), lds = p.kw > 1 ? waves * p.mt * 1024 : 0;
+#define MX_SKINNY(MT) if (p.mt == MT) mx_skinny_kernel<FA, FB, WIDE, MT><<<grid, waves * 64, lds, st>>>(g, p.kw);
+        MX_SKINNY(1) MX_SKINNY(2) MX_SKINNY(3) MX_SKINNY(4)
 #undef MX_SKINNY
     } else {
         const unsigned grid = (unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits);
         if constexpr (!WIDE) if (p.bm == 256) mx_tile_gemm_kernel<FA, FB, WIDE, 256, 256, 2><<<grid, 256, 0, st>>>(g);
         if (p.bm == 128) mx_tile_gemm_kernel<FA, FB, WIDE, 128, 128, 2><<<grid, 256, 0, st>>>(g);
+        if (p.bm == 64) mx_tile_gemm_kernel<FA, FB, WIDE, 64, 128, 2><<<grid, 256, 0, st>>>(g);
     }
     MX_LAUNCHED();
     if (g.part) {

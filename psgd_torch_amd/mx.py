@@ -82,12 +82,13 @@ def _ptr(t) -> Optional[int]:
 
 # (the calls below cost microseconds on the device at the smallest sizes: the host side avoids objects it does not need)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice          # (a tensor on the device is at hand: CUDA is initialised)
 
 
 def _launch(what, device, fn, *args):
     """fn(*args, current stream of `device`) with that device current."""
     i = device.index
-    if i == torch.cuda.current_device():
+    if i == _current_device():
         rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(i):
@@ -113,12 +114,12 @@ class MxTensor:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, int], fmt: str):
         bits = _fmt(fmt)
-        rows, cols = (int(d) for d in shape)
+        rows, cols = shape
         if rows < 0 or cols < 0:
             raise _bad(f"MxTensor shape {tuple(shape)}")
         wide = -(-cols // _PAD) * _PAD
         for what, t, n in (("codes", codes, wide * bits // 8), ("scales", scales, wide // _BLOCK)):
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or tuple(t.shape) != (rows, n) or not t.is_contiguous():
+            if not isinstance(t, torch.Tensor) or t.dtype is not torch.uint8 or t.shape != (rows, n) or not t.is_contiguous():
                 raise _bad(f"MxTensor {what}: a contiguous uint8 tensor of shape {(rows, n)} for a {rows} x {cols} matrix in {fmt}")
         if codes.device != scales.device:
             raise _bad(f"MxTensor codes live on {codes.device}, scales on {scales.device}")
@@ -161,15 +162,10 @@ def _mx(what, t, device=None) -> MxTensor:
 
 def _quantize(items, fmt, device):
     """items: [(x (2-D), noise or None, MxTensor of x or None, MxTensor of x transposed or None)] of one dtype, all with the same outputs."""
-    jobs = (L.MxTensorArg * len(items))()
-    for j, (x, noise, r, c) in zip(jobs, items):
-        j.x, j.rows, j.cols, j.ld = x.data_ptr(), x.shape[0], x.shape[1], _ld(x)
-        if noise is not None:
-            j.noise = noise.data_ptr()
-        if r is not None:
-            j.codes, j.scales = r.codes.data_ptr(), r.scales.data_ptr()
-        if c is not None:
-            j.codes_t, j.scales_t = c.codes.data_ptr(), c.scales.data_ptr()
+    jobs = (L.MxTensorArg * len(items))(*[
+        (x.data_ptr(), None if noise is None else noise.data_ptr(), None if r is None else r.codes.data_ptr(), None if r is None else r.scales.data_ptr(),
+         None if c is None else c.codes.data_ptr(), None if c is None else c.scales.data_ptr(), x.shape[0], x.shape[1], _ld(x))
+        for x, noise, r, c in items])
     _launch("mx_quantize", device, L.lib().psgdk_mx_quantize, len(items), jobs, _DTYPE[items[0][0].dtype], _FMT[fmt])
 
 
@@ -381,9 +377,8 @@ def refresh_mx_weights(weights: Sequence[MxWeight]) -> None:
             torch.autograd.graph.increment_version([t for q in (r, c) if q is not None for t in (q.codes, q.scales)])
 
 
-def _restore(ctx, i, shape, fmt) -> MxTensor:
-    codes, scales = ctx.saved_tensors[i:i + 2]
-    return MxTensor._of(codes, scales, shape, fmt)
+def _restore(saved, i, shape, fmt) -> MxTensor:
+    return MxTensor._of(saved[i], saved[i + 1], shape, fmt)
 
 
 def _weight_args(x, weight, fmt, grad_fmt):
@@ -407,13 +402,13 @@ def _tracked(*ts):
     return ts if torch.is_grad_enabled() else tuple(None if t is None else t.detach() for t in ts)
 
 
-def _product_grads(ctx, dout, need_x, need_w, cols_at, act_at, x_dtype):
+def _product_grads(ctx, saved, dout, need_x, need_w, cols_at, act_at, x_dtype):
     """(gradient of the product's input in x_dtype, of the weight) from dout."""
     n, k = ctx.weight_shape
     d2 = _rows("gradient", dout)
     dr, dc = _rounded(d2, ctx.grad_fmt, need_x, need_w)
-    dx = _matmul(dr, _restore(ctx, cols_at, (k, n), ctx.weight_fmt), x_dtype, _DTYPE[x_dtype]) if need_x else None
-    dw = _matmul(dc, _restore(ctx, act_at, (k, d2.shape[0]), ctx.fmt), ctx.weight_dtype, _DTYPE[ctx.weight_dtype]) if need_w else None
+    dx = _matmul(dr, _restore(saved, cols_at, (k, n), ctx.weight_fmt), x_dtype, _DTYPE[x_dtype]) if need_x else None
+    dw = _matmul(dc, _restore(saved, act_at, (k, d2.shape[0]), ctx.fmt), ctx.weight_dtype, _DTYPE[ctx.weight_dtype]) if need_w else None
     return dx, dw
 
 
@@ -438,7 +433,7 @@ class _Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx, dw = _product_grads(ctx, dout, need_x, need_w, 0, 2 if need_x else 0, ctx.x_dtype)
+        dx, dw = _product_grads(ctx, ctx.saved_tensors, dout, need_x, need_w, 0, 2 if need_x else 0, ctx.x_dtype)
         return (dx.view(ctx.x_shape) if need_x else None), dw, None, None, None
 
 
@@ -467,11 +462,12 @@ class _NormLinear(torch.autograd.Function):
         need_s = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         need_g, need_w = ctx.needs_input_grad[2:4]
         need_y = need_s or need_g
-        s, inv, gain = ctx.saved_tensors[:3]
+        saved = ctx.saved_tensors
+        s, inv, gain = saved[:3]
         dx = dg = dw = None
         if dout is not None:
             # (the gradient of y stays in fp32 between the two kernels: one rounding, at dx)
-            dy, dw = _product_grads(ctx, dout, need_y, need_w, 3, 5 if need_y else 3, torch.float32)
+            dy, dw = _product_grads(ctx, saved, dout, need_y, need_w, 3, 5 if need_y else 3, torch.float32)
             if need_y:
                 dx, dg = _norm_backward(dy.view(s.shape), s, gain, inv, ds)
                 dg = dg.to(gain.dtype)
