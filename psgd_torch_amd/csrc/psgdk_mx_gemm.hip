@@ -1,11 +1,12 @@
 // psgdk_mx_gemm.hip -- psgdk_mx_matmul (include/psgdk.h, "microscaled numbers"): argument checks, choice of kernel, launches.
+#include <cmath>
 #include "mx_host.hiph"
 #include "gemm_mx.hiph"
 
 // a 32-bit output with an 8-bit operand: fp32 sums through bf16 products (gemm_mx.hiph)
 static bool mx_wide(int a_fmt, int b_fmt, int out_dtype) { return out_dtype == PSGDK_F32 && (a_fmt == PSGDK_MX_FP8 || b_fmt == PSGDK_MX_FP8); }
 struct MxPlan { bool skinny; int mt, kw, bm, bn, splits; };
-static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, bool wide) {
+static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, int a_fmt, int b_fmt, bool wide) {
     MxPlan p{};
     p.splits = 1;
     // Few rows: the kernel without LDS reads A anew for every 16 rows of B, the tiles once for 128.  Measured (fp8 x fp4, us, without / tiles): M = 5:
@@ -19,11 +20,24 @@ static MxPlan mx_plan(int64_t M, int64_t N, int64_t KS, bool wide) {
         while (p.kw < 8 && (N + 15) / 16 * p.kw < 2048 && p.kw < KS) p.kw *= 2;
         return p;
     }
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256);
-    p.bm = p.bn = big >= 256 && !wide ? 256 : 128;
-    if (M <= 64) p.bm = 64;
-    const int64_t tiles = ((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
-    while (p.splits < 16 && tiles * p.splits * 2 <= 512 && KS / (p.splits * 2) >= 2) p.splits *= 2;
+    // Tiles: the size and the number of splits of K with the smallest estimated time.  Microseconds for 256 elements of K, measured at 4096 x 4096 and
+    // 2048 x 2048: a workgroup alone on its CU, and (128 rows) each of two; for the prologue and stores of a round of tiles; a split adds a launch and
+    // fp32 sums that are written and read once.
+    const bool four = a_fmt == PSGDK_MX_FP4 && b_fmt == PSGDK_MX_FP4;
+    const double big = four ? 1.9 : 2.8, alone = wide ? 1.9 : four ? 0.8 : 1.3, pair = wide ? 3.0 : four ? 1.04 : 1.67;
+    double best = 1e30;
+    for (int bm = 256; bm >= 64; bm /= 2) {
+        if ((bm == 64) != (M <= 64) || (bm == 256 && wide)) continue;
+        const int bn = bm == 256 ? 256 : 128;
+        const double tiles = (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+        for (int splits = 1; splits <= 16 && (splits == 1 || splits * 2 <= KS); splits *= 2) {
+            const double wgs = tiles * splits, blocks = (double)((KS + splits - 1) / splits);
+            double t = bm == 256 ? std::ceil(wgs / 256) * (blocks * big + 6.0)
+                                 : (wgs <= 256 ? blocks * alone + 2.2 : std::ceil(wgs / 512) * (blocks * pair + 2.2)) * (bm == 64 ? 0.7 : 1.0);
+            if (splits > 1) t += 4.0 + (double)M * N * splits * 8 / 4.5e6;
+            if (t < best) { best = t; p.bm = bm; p.bn = bn; p.splits = splits; }
+        }
+    }
     return p;
 }
 
@@ -56,7 +70,7 @@ extern "C" {
 int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int out_dtype, size_t* bytes) {
     if (m < 0 || n < 0 || k < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim || !bytes) return PSGDK_ERR_INVALID;
     if (!mx_fmt_ok(a_fmt) || !mx_fmt_ok(b_fmt) || !mx_dtype_ok(out_dtype)) return PSGDK_ERR_INVALID;
-    const MxPlan p = mx_plan(m, n, mx_pad(k) / MX_PAD, mx_wide(a_fmt, b_fmt, out_dtype));
+    const MxPlan p = mx_plan(m, n, mx_pad(k) / MX_PAD, a_fmt, b_fmt, mx_wide(a_fmt, b_fmt, out_dtype));
     *bytes = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
     return PSGDK_OK;
 }
@@ -72,7 +86,7 @@ int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_
     if (!mx_aligned(a_codes, 16) || !mx_aligned(b_codes, 16) || !mx_aligned(a_scales, 8) || !mx_aligned(b_scales, 8)) return PSGDK_ERR_INVALID;
     const int64_t KS = mx_pad(k) / MX_PAD;
     const bool wide = mx_wide(a_fmt, b_fmt, out_dtype);
-    const MxPlan p = mx_plan(m, n, KS, wide);
+    const MxPlan p = mx_plan(m, n, KS, a_fmt, b_fmt, wide);
     const size_t need = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
     if (need && (!work || work_bytes < need || !mx_aligned(work, 16))) return PSGDK_ERR_INVALID;
     const int64_t tm = p.skinny ? 1 : (m + p.bm - 1) / p.bm, tn = p.skinny ? 1 : (n + p.bn - 1) / p.bn;
