@@ -12,8 +12,8 @@ static int mx_by_dtype(int d, F&& f) {
 template <typename T, int FMT, bool NOISE>
 static int mx_launch_round(const MxJobs& a, unsigned grid, bool rows, bool cols, hipStream_t st) {
     if (!cols) mx_rows_kernel<T, FMT, NOISE><<<grid, 256, 0, st>>>(a);
-    else if (rows) mx_tile_kernel<T, FMT, true, NOISE, false><<<grid, 256, 0, st>>>(a, MxNormArgs{nullptr, nullptr, 0});
-    else mx_tile_kernel<T, FMT, false, NOISE, false><<<grid, 256, 0, st>>>(a, MxNormArgs{nullptr, nullptr, 0});
+    else if (rows) mx_tile_kernel<T, FMT, true, NOISE, false><<<grid, 128 * sizeof(T), 0, st>>>(a, MxNormArgs{nullptr, nullptr, 0});
+    else mx_tile_kernel<T, FMT, false, NOISE, false><<<grid, 128 * sizeof(T), 0, st>>>(a, MxNormArgs{nullptr, nullptr, 0});
     MX_LAUNCHED();
     return PSGDK_OK;
 }
@@ -83,7 +83,6 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
         if (!mx_aligned(q.x, mx_size(dtype)) || !mx_aligned(q.codes, 16) || !mx_aligned(q.codes_t, 16)) return PSGDK_ERR_INVALID;
     }
     const hipStream_t st = (hipStream_t)stream;
-    const int tc = 256 / mx_size(dtype);
     for (int i = 0; i < count;) {
         MxJobs a;
         a.n = 0;
@@ -91,8 +90,8 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
         for (; i < count && a.n < MX_JOBS; ++i) {
             const psgdk_mx_tensor& q = t[i];
             if (q.rows == 0 || q.cols == 0) continue;
-            // rows: units of 256 elements, 8 a workgroup; tiles: 128 rows x tc columns over the padded extent of what is written
-            const int64_t units = mx_pad(q.cols) / MX_PAD, tiles_n = (rows ? mx_pad(q.cols) : q.cols + tc - 1) / tc;
+            // rows: units of 256 elements, 8 a workgroup; tiles: 128 x 128 over the padded extent of what is written
+            const int64_t units = mx_pad(q.cols) / MX_PAD, tiles_n = (rows ? mx_pad(q.cols) : q.cols + 127) / 128;
             const int64_t need = cols ? mx_pad(q.rows) / 128 * tiles_n : (q.rows * units + 7) / 8;
             if (need > (1ll << 28)) return PSGDK_ERR_UNSUPPORTED;
             if (wgs + need > (1ll << 28)) break;
@@ -141,7 +140,7 @@ int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int
     if (!mx_aligned(x, size) || !mx_aligned(residual, size) || !mx_aligned(s, size) || !mx_aligned(gain, mx_size(gain_dtype)) || !mx_aligned(inv, 4) ||
         !mx_aligned(codes, 16) || !mx_aligned(codes_t, 16)) return PSGDK_ERR_INVALID;
     const hipStream_t st = (hipStream_t)stream;
-    const int64_t tiles_n = (cols + 256 / size - 1) / (256 / size), tiles = mx_pad(rows) / 128 * tiles_n;
+    const int64_t tiles_n = (cols + 127) / 128, tiles = mx_pad(rows) / 128 * tiles_n;
     if (codes_t && tiles > (1ll << 28)) return PSGDK_ERR_UNSUPPORTED;
     return mx_by_dtype(dtype, [&](auto* e) {
         using T = std::remove_pointer_t<decltype(e)>;
@@ -157,7 +156,7 @@ int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int
             a.j[0] = MxJob{residual ? s : x, nullptr, nullptr, nullptr, (uint8_t*)codes_t, (uint8_t*)scales_t, cols, (int)rows, (int)cols, 0u,
                            FastDiv::make((unsigned)tiles_n)};
             const MxNormArgs n{inv, gain, gain_dtype};
-#define MX_NT(F) mx_tile_kernel<T, F, false, false, true><<<(unsigned)tiles, 256, 0, st>>>(a, n)
+#define MX_NT(F) mx_tile_kernel<T, F, false, false, true><<<(unsigned)tiles, 128 * sizeof(T), 0, st>>>(a, n)
             if (fmt == PSGDK_MX_FP4) MX_NT(4);
             else MX_NT(8);
 #undef MX_NT
