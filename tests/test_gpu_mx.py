@@ -544,6 +544,29 @@ def test_training_with_kwns4(p):
             _same(m.cols, O.quantize(w.detach().cpu().t(), "fp4"), "cols")
 
 
+def test_layers_on_no_tokens(p):
+    w, gain = torch.randn(40, 64, device=DEV, requires_grad=True), torch.ones(64, device=DEV, requires_grad=True)
+    x = torch.zeros(0, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    out, s = p.mx_norm_linear(x, gain, p.MxWeight(w), x)
+    gx, gg, gw = torch.autograd.grad((out.float().sum() + s.float().sum()), (x, gain, w))
+    assert out.shape == (0, 40) and gx.shape == (0, 64) and not gg.any() and not gw.any() and gw.shape == w.shape
+    (gw,) = torch.autograd.grad(p.mx_linear(x, p.MxWeight(w)).float().sum(), w)
+    assert not gw.any()
+
+
+def test_one_tensor_as_input_and_residual(p):
+    """s = 2 x: both paths' gradients add up; the graph is walked twice."""
+    g = torch.Generator().manual_seed(36)
+    x, w, gain = torch.randn(6, 64, generator=g), torch.randn(32, 64, generator=g), torch.ones(64)
+    d = torch.randn(6, 32, generator=g)
+    _, _, dx, _, dw = _layer_reference(x, x, gain, w, d, None, "fp8", "fp8", "fp4")
+    xg, wg = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    out, _ = p.mx_norm_linear(xg, gain.to(DEV), p.MxWeight(wg), xg)
+    for _ in range(2):
+        gx, gw = torch.autograd.grad(out, (xg, wg), d.to(DEV), retain_graph=True)
+        assert float((gx.cpu().double() - 2 * dx).norm() / dx.norm()) < 3e-3 and float((gw.cpu().double() - dw).norm() / dw.norm()) < 5e-3
+
+
 # ---- streams, graphs, size ---------------------------------------------------------------------------------------------------------------
 
 def test_another_stream(p):
@@ -557,6 +580,64 @@ def test_another_stream(p):
         got = p.mx_matmul(p.mx_quantize(y * 0.5, "fp8"), w)
     st.synchronize()
     assert torch.equal(got, want)
+
+
+def test_two_streams_at_once(p):
+    """The same operators on two streams, interleaved: each has its own outputs and workspaces."""
+    sets = []
+    for seed, (m, n, k) in ((1, (300, 200, 5000)), (2, (700, 130, 3000))):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        sets.append((torch.randn(m, k, generator=g, device=DEV), p.mx_quantize(torch.randn(n, k, generator=g, device=DEV)), torch.ones(k, device=DEV)))
+
+    def run(x, w, gain):
+        y, s, inv = p.rms_norm_mx(x, gain, x, which="both")
+        return p.mx_matmul(y[0], w, out_dtype=torch.float32), p.mx_dequantize(y[1]), *p.rms_norm_mx_backward(x, s, gain, inv)
+    want = [run(*t) for t in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for a, b in zip(r, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_layer_captured_with_its_backward(p):
+    """Forward and backward of the differentiable layer in a graph (torch.autograd.grad inside the capture), the weight renewed between replays."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x, res, dout = (torch.randn(130, n, generator=g, device=DEV).to(torch.bfloat16) for n in (96, 96, 70))
+    w = torch.nn.Parameter(torch.randn(70, 96, generator=g, device=DEV))
+    gain = torch.ones(96, device=DEV)
+    weight = p.MxWeight(w)
+
+    def run():
+        leaves = [x.detach().requires_grad_(), res.detach().requires_grad_(), gain.detach().requires_grad_()]
+        out, s = p.mx_norm_linear(leaves[0], leaves[2], weight, leaves[1])
+        return out.detach(), s.detach(), *torch.autograd.grad(out, [*leaves, w], dout)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run()
+    for i in range(4):
+        with torch.no_grad():
+            w.add_(0.1 * torch.randn_like(w))
+            x.copy_(torch.randn_like(x))
+        weight.refresh()
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in outs]
+        for a, b in zip(kept, run()):
+            assert torch.equal(a, b), i
 
 
 def test_graph_replays(p):

@@ -157,3 +157,52 @@ def test_oracle_rounding():
     x = torch.full((1, 32), 1.0)
     x[0, 5] = math.inf
     assert torch.isnan(O.rounded(x, "fp4")).all()
+
+
+def _kernels():
+    """{kernel: its instructions} of the library's gfx950 code objects."""
+    import os
+    import re
+    import subprocess
+    import tempfile
+    from psgd_torch_amd import _lib
+    llvm = "/opt/rocm/lib/llvm/bin"
+    out = {}
+    with tempfile.TemporaryDirectory() as tmp:
+        fat = os.path.join(tmp, "fat")
+        subprocess.run([f"{llvm}/llvm-objcopy", "-O", "binary", "--only-section=.hip_fatbin", _lib.LIB_PATH, fat], check=True)
+        data = open(fat, "rb").read()
+        magic = b"__CLANG_OFFLOAD_BUNDLE__"
+        starts = [m.start() for m in re.finditer(magic, data)]
+        for i, a in enumerate(starts):
+            part, co = os.path.join(tmp, f"b{i}"), os.path.join(tmp, f"c{i}")
+            open(part, "wb").write(data[a:starts[i + 1] if i + 1 < len(starts) else len(data)])
+            subprocess.run([f"{llvm}/clang-offload-bundler", "--unbundle", "--type=o", f"--input={part}", "--targets=hipv4-amdgcn-amd-amdhsa--gfx950", f"--output={co}"],
+                           check=True, capture_output=True)
+            text = subprocess.run([f"{llvm}/llvm-objdump", "-d", "--no-show-raw-insn", "--no-leading-addr", co], check=True, capture_output=True, text=True).stdout
+            for f in re.split(r"\n(?=<)", text):
+                m = re.match(r"<([^>]+)>:", f)
+                if m:
+                    out[m.group(1)] = [line.split("//")[0].strip() for line in f.split("\n")[1:]]
+    return out
+
+
+def test_main_loops_of_the_large_tiles(lib):
+    """The large tile's products are inline assembly on accumulators that the compiler must not touch while they are in flight: between the first and the last
+    matrix instruction nothing may read, move or spill an accumulation register, nor go to scratch; behind the last one come the waits."""
+    found = 0
+    for name, code in _kernels().items():
+        if "mx_tile_gemm_kernel" not in name or "Li256ELi256E" not in name:
+            continue
+        found += 1
+        mfma = [i for i, c in enumerate(code) if c.startswith("v_mfma")]
+        assert len(mfma) == 128, (name, len(mfma))
+        for c in code[mfma[0]:mfma[-1]]:
+            assert not c.startswith(("v_accvgpr", "scratch_")), (name, c)
+            assert c.startswith("v_mfma") or not any(op.startswith(("a[", "a0", "a1", "a2")) for op in c.replace(",", " ").split()[1:]), (name, c)
+        behind = code[mfma[-1] + 1:]
+        waits = [i for i, c in enumerate(behind) if c.startswith("s_nop 15")][:2]
+        assert len(waits) == 2 and all(c.startswith("s_") for c in behind[:waits[1]]), name
+        loop = [i for i, c in enumerate(behind[:waits[0]]) if c.startswith("s_cbranch")]
+        assert len(loop) == 1 and not any(c.startswith("s_branch") for c in behind[:waits[1]]), name      # the loop's own end, then straight on
+    assert found == 4, found
