@@ -30,6 +30,7 @@ _FMT = {"fp4": 4, "fp8": 8}
 _DTYPE = {torch.bfloat16: L.BF16, torch.float32: L.F32, torch.float16: L.F16}
 _PAD = 256          # elements a stored row is a multiple of
 _BLOCK = 32
+_NONE = (None, None)
 NORM_MAX_COLS = 16384
 
 
@@ -110,7 +111,7 @@ class MxTensor:
     of its byte; scales: uint8 (rows, pad(cols) / 32), 2^(byte - 127), 255 for NaN; pad: the next multiple of 256.  Elements behind `cols` are zero
     codes (they take part in products).  Holds no autograd history."""
 
-    __slots__ = ("codes", "scales", "shape", "fmt")
+    __slots__ = ("shape", "fmt", "device", "_codes", "_scales", "_buffer", "_at", "_ptrs")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: Tuple[int, int], fmt: str):
         bits = _fmt(fmt)
@@ -121,28 +122,41 @@ class MxTensor:
         for what, t, n in (("codes", codes, wide * bits // 8), ("scales", scales, wide // _BLOCK)):
             if not isinstance(t, torch.Tensor) or t.dtype is not torch.uint8 or t.shape != (rows, n) or not t.is_contiguous():
                 raise _bad(f"MxTensor {what}: a contiguous uint8 tensor of shape {(rows, n)} for a {rows} x {cols} matrix in {fmt}")
-        if codes.device != scales.device:
-            raise _bad(f"MxTensor codes live on {codes.device}, scales on {scales.device}")
-        if codes.data_ptr() % 16 or scales.data_ptr() % 8:
+        device = codes.device
+        if device != scales.device:
+            raise _bad(f"MxTensor codes live on {device}, scales on {scales.device}")
+        ptrs = codes.data_ptr(), scales.data_ptr()
+        if ptrs[0] % 16 or ptrs[1] % 8:
             raise _bad("MxTensor codes need 16-byte, scales 8-byte alignment")
-        self.codes, self.scales, self.shape, self.fmt = codes, scales, (rows, cols), fmt
+        self.shape, self.fmt, self.device = (rows, cols), fmt, device
+        self._codes, self._scales, self._buffer, self._at, self._ptrs = codes, scales, None, 0, ptrs
 
     @classmethod
     def empty(cls, rows: int, cols: int, fmt: str, device) -> "MxTensor":
+        """A new one in one piece of memory; codes and scales become tensors (views of it) when somebody asks for them."""
         wide = -(-cols // _PAD) * _PAD
-        return cls._of(torch.empty((rows, wide * _fmt(fmt) // 8), dtype=torch.uint8, device=device),
-                       torch.empty((rows, wide // _BLOCK), dtype=torch.uint8, device=device), (rows, cols), fmt)
-
-    @classmethod
-    def _of(cls, codes, scales, shape, fmt) -> "MxTensor":
-        """From parts that are known to fit."""
+        n, m = rows * (wide * _fmt(fmt) // 8), rows * (wide // _BLOCK)          # (a stored row of codes is a multiple of 128 bytes)
         t = object.__new__(cls)
-        t.codes, t.scales, t.shape, t.fmt = codes, scales, shape, fmt
+        t._buffer = torch.empty(n + m, dtype=torch.uint8, device=device)
+        base = t._buffer.data_ptr()
+        t.shape, t.fmt, t.device, t._codes, t._scales, t._at, t._ptrs = (rows, cols), fmt, t._buffer.device, None, None, n, (base, base + n)
         return t
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._buffer[:self._at].view(self.shape[0], -(-self.shape[1] // _PAD) * _PAD * _FMT[self.fmt] // 8)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._buffer[self._at:].view(self.shape[0], -(-self.shape[1] // _PAD) * _PAD // _BLOCK)
+        return self._scales
+
+    def _memory(self) -> List[torch.Tensor]:
+        """The tensors that hold it (autograd saves these, and sees by them whether it was written again)."""
+        return [self._codes, self._scales] if self._buffer is None else [self._buffer]
 
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
         return mx_dequantize(self, dtype)
@@ -154,7 +168,10 @@ class MxTensor:
 def _mx(what, t, device=None) -> MxTensor:
     if not isinstance(t, MxTensor):
         raise _bad(f"{what} is not an MxTensor")
-    _tensor(what, t.codes, device)
+    if t.device.type != "cuda":
+        raise _bad(f"{what} lives on {t.device}: MX operators need tensors on a ROCm device; there is no CPU fallback")
+    if device is not None and t.device != device:
+        raise _bad(f"{what} lives on {t.device}, the others on {device}")
     return t
 
 
@@ -163,8 +180,8 @@ def _mx(what, t, device=None) -> MxTensor:
 def _quantize(items, fmt, device):
     """items: [(x (2-D), noise or None, MxTensor of x or None, MxTensor of x transposed or None)] of one dtype, all with the same outputs."""
     jobs = (L.MxTensorArg * len(items))(*[
-        (x.data_ptr(), None if noise is None else noise.data_ptr(), None if r is None else r.codes.data_ptr(), None if r is None else r.scales.data_ptr(),
-         None if c is None else c.codes.data_ptr(), None if c is None else c.scales.data_ptr(), x.shape[0], x.shape[1], _ld(x))
+        (x.data_ptr(), None if noise is None else noise.data_ptr(), *(_NONE if r is None else r._ptrs), *(_NONE if c is None else c._ptrs),
+         x.shape[0], x.shape[1], _ld(x))
         for x, noise, r, c in items])
     _launch("mx_quantize", device, L.lib().psgdk_mx_quantize, len(items), jobs, _DTYPE[items[0][0].dtype], _FMT[fmt])
 
@@ -205,7 +222,7 @@ def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
     _mx("t", t)
     code = _dtype("out", dtype)
     out = torch.empty(t.shape, dtype=dtype, device=t.device)
-    _launch("mx_dequantize", out.device, L.lib().psgdk_mx_dequantize, t.codes.data_ptr(), t.scales.data_ptr(), *t.shape, _FMT[t.fmt], out.data_ptr(), code)
+    _launch("mx_dequantize", out.device, L.lib().psgdk_mx_dequantize, *t._ptrs, *t.shape, _FMT[t.fmt], out.data_ptr(), code)
     return out
 
 
@@ -218,7 +235,7 @@ def mx_matmul(a: MxTensor, b: MxTensor, *, out_dtype: torch.dtype = torch.bfloat
     that is taken for 16-bit outputs, whose own rounding is a hundred times larger.  An fp32 output has fp32 sums throughout, at half the rate
     (elements below 2^-126 count as zero there)."""
     _mx("a", a)
-    _mx("b", b, a.codes.device)
+    _mx("b", b, a.device)
     if a.shape[1] != b.shape[1]:
         raise _bad(f"mx_matmul: a is {a.shape[0]} x {a.shape[1]}, b is {b.shape[0]} x {b.shape[1]}: both are contracted along their rows")
     return _matmul(a, b, out_dtype, _dtype("out", out_dtype))
@@ -226,12 +243,11 @@ def mx_matmul(a: MxTensor, b: MxTensor, *, out_dtype: torch.dtype = torch.bfloat
 
 def _matmul(a, b, out_dtype, code):
     (m, k), n = a.shape, b.shape[0]
-    device = a.codes.device
+    device = a.device
     out = torch.empty((m, n), dtype=out_dtype, device=device)
     wb = _work_bytes("psgdk_mx_matmul_work_bytes", m, n, k, _FMT[a.fmt], _FMT[b.fmt], code)
     work = torch.empty(wb, dtype=torch.uint8, device=device) if wb else None
-    _launch("mx_matmul", device, L.lib().psgdk_mx_matmul, a.codes.data_ptr(), a.scales.data_ptr(), m, _FMT[a.fmt], b.codes.data_ptr(), b.scales.data_ptr(), n,
-            _FMT[b.fmt], k, out.data_ptr(), code, work.data_ptr() if wb else None, wb)
+    _launch("mx_matmul", device, L.lib().psgdk_mx_matmul, *a._ptrs, m, _FMT[a.fmt], *b._ptrs, n, _FMT[b.fmt], k, out.data_ptr(), code, work.data_ptr() if wb else None, wb)
     return out
 
 
@@ -286,8 +302,7 @@ def _norm(x, gain, residual, eps, fmt, rows, cols):
     r = MxTensor.empty(n, d, fmt, device) if rows else None
     c = MxTensor.empty(d, n, fmt, device) if cols else None
     _launch("rms_norm_mx", device, L.lib().psgdk_rms_norm_mx, x.data_ptr(), res, gain.data_ptr(), _DTYPE[gain.dtype], n, d, _DTYPE[x.dtype], eps, _FMT[fmt],
-            s.data_ptr(), inv.data_ptr(), r.codes.data_ptr() if rows else None, r.scales.data_ptr() if rows else None,
-            c.codes.data_ptr() if cols else None, c.scales.data_ptr() if cols else None)
+            s.data_ptr(), inv.data_ptr(), *(r._ptrs if rows else _NONE), *(c._ptrs if cols else _NONE))
     return r, c, s, inv
 
 
@@ -374,11 +389,7 @@ def refresh_mx_weights(weights: Sequence[MxWeight]) -> None:
     for (device, _, fmt, both), items in groups.items():
         _quantize(items, fmt, device)
         for _, _, r, c in items:
-            torch.autograd.graph.increment_version([t for q in (r, c) if q is not None for t in (q.codes, q.scales)])
-
-
-def _restore(saved, i, shape, fmt) -> MxTensor:
-    return MxTensor._of(saved[i], saved[i + 1], shape, fmt)
+            torch.autograd.graph.increment_version([t for q in (r, c) if q is not None for t in q._memory()])
 
 
 def _weight_args(x, weight, fmt, grad_fmt):
@@ -402,14 +413,21 @@ def _tracked(*ts):
     return ts if torch.is_grad_enabled() else tuple(None if t is None else t.detach() for t in ts)
 
 
-def _product_grads(ctx, saved, dout, need_x, need_w, cols_at, act_at, x_dtype):
+def _product_grads(ctx, dout, need_x, need_w, x_dtype):
     """(gradient of the product's input in x_dtype, of the weight) from dout."""
-    n, k = ctx.weight_shape
-    d2 = _rows("gradient", dout)
-    dr, dc = _rounded(d2, ctx.grad_fmt, need_x, need_w)
-    dx = _matmul(dr, _restore(saved, cols_at, (k, n), ctx.weight_fmt), x_dtype, _DTYPE[x_dtype]) if need_x else None
-    dw = _matmul(dc, _restore(saved, act_at, (k, d2.shape[0]), ctx.fmt), ctx.weight_dtype, _DTYPE[ctx.weight_dtype]) if need_w else None
+    dr, dc = _rounded(_rows("gradient", dout), ctx.grad_fmt, need_x, need_w)
+    dx = _matmul(dr, ctx.cols, x_dtype, _DTYPE[x_dtype]) if need_x else None
+    dw = _matmul(dc, ctx.act, ctx.weight_dtype, _DTYPE[ctx.weight_dtype]) if need_w else None
     return dx, dw
+
+
+def _keep(ctx, weight, param, act, need_x, need_w, grad_fmt, *more):
+    """What the backward pass needs: the MX forms on ctx, the memory they lie in saved, so that autograd refuses what was written again."""
+    ctx.cols, ctx.act = weight.cols if need_x else None, act if need_w else None
+    if need_x:
+        _need_cols(weight)
+    ctx.save_for_backward(*more, *(weight.cols._memory() if need_x else ()), *(act._memory() if need_w else ()))
+    ctx.weight_dtype, ctx.grad_fmt = param.dtype, grad_fmt
 
 
 class _Linear(torch.autograd.Function):
@@ -418,14 +436,7 @@ class _Linear(torch.autograd.Function):
         need_x, need_w = ctx.needs_input_grad[:2]
         xr, xc = _rounded(_rows("x", x), fmt, True, need_w)
         out = _matmul(xr, weight.rows, x.dtype, _DTYPE[x.dtype])
-        saved = []
-        if need_x:
-            _need_cols(weight)
-            saved += [weight.cols.codes, weight.cols.scales]
-        if need_w:
-            saved += [xc.codes, xc.scales]
-        ctx.save_for_backward(*saved)
-        ctx.weight_shape, ctx.weight_fmt, ctx.weight_dtype, ctx.fmt, ctx.grad_fmt = weight.rows.shape, weight.fmt, param.dtype, fmt, grad_fmt
+        _keep(ctx, weight, param, xc, need_x, need_w, grad_fmt)
         ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
         return out if x.dim() == 2 else out.view(*x.shape[:-1], weight.rows.shape[0])
 
@@ -433,7 +444,8 @@ class _Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         need_x, need_w = ctx.needs_input_grad[:2]
-        dx, dw = _product_grads(ctx, ctx.saved_tensors, dout, need_x, need_w, 0, 2 if need_x else 0, ctx.x_dtype)
+        ctx.saved_tensors                                # (raises where a kept form was renewed since)
+        dx, dw = _product_grads(ctx, dout, need_x, need_w, ctx.x_dtype)
         return (dx.view(ctx.x_shape) if need_x else None), dw, None, None, None
 
 
@@ -444,14 +456,7 @@ class _NormLinear(torch.autograd.Function):
         need_g, need_w = ctx.needs_input_grad[2:4]
         yr, yc, s, inv = _norm(x, gain, residual, eps, fmt, True, need_w)
         out = _matmul(yr, weight.rows, x.dtype, _DTYPE[x.dtype])
-        saved = [s, inv, gain]
-        if need_s or need_g:
-            _need_cols(weight)
-            saved += [weight.cols.codes, weight.cols.scales]
-        if need_w:
-            saved += [yc.codes, yc.scales]
-        ctx.save_for_backward(*saved)
-        ctx.weight_shape, ctx.weight_fmt, ctx.weight_dtype, ctx.fmt, ctx.grad_fmt = weight.rows.shape, weight.fmt, param.dtype, fmt, grad_fmt
+        _keep(ctx, weight, param, yc, need_s or need_g, need_w, grad_fmt, s, inv, gain)
         ctx.set_materialize_grads(False)
         out = out if x.dim() == 2 else out.view(*x.shape[:-1], weight.rows.shape[0])
         return out if residual is None else (out, s)
@@ -462,12 +467,11 @@ class _NormLinear(torch.autograd.Function):
         need_s = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         need_g, need_w = ctx.needs_input_grad[2:4]
         need_y = need_s or need_g
-        saved = ctx.saved_tensors
-        s, inv, gain = saved[:3]
+        s, inv, gain = ctx.saved_tensors[:3]
         dx = dg = dw = None
         if dout is not None:
             # (the gradient of y stays in fp32 between the two kernels: one rounding, at dx)
-            dy, dw = _product_grads(ctx, saved, dout, need_y, need_w, 3, 5 if need_y else 3, torch.float32)
+            dy, dw = _product_grads(ctx, dout, need_y, need_w, torch.float32)
             if need_y:
                 dx, dg = _norm_backward(dy.view(s.shape), s, gain, inv, ds)
                 dg = dg.to(gain.dtype)
