@@ -109,7 +109,7 @@ def _work_bytes(name, *sizes) -> int:
 class MxTensor:
     """A rows x cols matrix in MX form, blocks along its rows.  codes: uint8 (rows, pad(cols) * bits / 8), in 4 bits the even element in the low half
     of its byte; scales: uint8 (rows, pad(cols) / 32), 2^(byte - 127), 255 for NaN; pad: the next multiple of 256.  Elements behind `cols` are zero
-    codes (they take part in products).  Holds no autograd history."""
+    codes under finite scales (they take part in products).  Holds no autograd history."""
 
     __slots__ = ("shape", "fmt", "device", "_codes", "_scales", "_buffer", "_at", "_ptrs")
 
@@ -153,6 +153,10 @@ class MxTensor:
         if self._scales is None:
             self._scales = self._buffer[self._at:].view(self.shape[0], -(-self.shape[1] // _PAD) * _PAD // _BLOCK)
         return self._scales
+
+    def __reduce__(self):
+        """Copies and pickles go through the constructor: the addresses belong to this object's memory."""
+        return MxTensor, (self.codes, self.scales, self.shape, self.fmt)
 
     def _memory(self) -> List[torch.Tensor]:
         """The tensors that hold it (autograd saves these, and sees by them whether it was written again)."""

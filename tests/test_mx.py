@@ -206,3 +206,24 @@ def test_main_loops_of_the_large_tiles(lib):
         loop = [i for i, c in enumerate(behind[:waits[0]]) if c.startswith("s_cbranch")]
         assert len(loop) == 1 and not any(c.startswith("s_branch") for c in behind[:waits[1]]), name      # the loop's own end, then straight on
     assert found == 4, found
+
+
+def test_copies_and_pickles_have_addresses_of_their_own():
+    import copy
+    import io
+
+    import psgd_torch_amd as p
+    one = p.MxTensor.empty(4, 300, "fp8", "cpu")
+    one.codes.random_(0, 256)
+    one.scales.random_(0, 255)
+    two = p.MxTensor(one.codes.clone(), one.scales.clone(), (4, 300), "fp8")
+    for t in (one, two):
+        file = io.BytesIO()
+        torch.save(t, file)
+        file.seek(0)
+        for c in (copy.deepcopy(t), torch.load(file, weights_only=False)):
+            assert (c.shape, c.fmt, c.device) == (t.shape, t.fmt, t.device)
+            assert torch.equal(c.codes, t.codes) and torch.equal(c.scales, t.scales)
+            assert c._ptrs == (c.codes.data_ptr(), c.scales.data_ptr()) and not set(c._ptrs) & set(t._ptrs)
+        c = copy.copy(t)                                     # the same memory, held by the copy too
+        assert c._ptrs == t._ptrs == (c.codes.data_ptr(), c.scales.data_ptr())
