@@ -83,6 +83,7 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
         if (!mx_aligned(q.x, mx_size(dtype)) || !mx_aligned(q.codes, 16) || !mx_aligned(q.codes_t, 16)) return PSGDK_ERR_INVALID;
     }
     const hipStream_t st = (hipStream_t)stream;
+    const int64_t most = kMaxThreads / (cols ? 128 * mx_size(dtype) : 256);      // workgroups of a launch
     for (int i = 0; i < count;) {
         MxJobs a;
         a.n = 0;
@@ -93,8 +94,8 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
             // rows: units of 256 elements, 8 a workgroup; tiles: 128 x 128 over the padded extent of what is written
             const int64_t units = mx_pad(q.cols) / MX_PAD, tiles_n = (rows ? mx_pad(q.cols) : q.cols + 127) / 128;
             const int64_t need = cols ? mx_pad(q.rows) / 128 * tiles_n : (q.rows * units + 7) / 8;
-            if (need > (1ll << 28)) return PSGDK_ERR_UNSUPPORTED;
-            if (wgs + need > (1ll << 28)) break;
+            if (need > most) return PSGDK_ERR_UNSUPPORTED;
+            if (wgs + need > most) break;
             MxJob& j = a.j[a.n++];
             j = MxJob{q.x, (const uint8_t*)q.noise, (uint8_t*)q.codes, (uint8_t*)q.scales, (uint8_t*)q.codes_t, (uint8_t*)q.scales_t, q.ld, (int)q.rows,
                       (int)q.cols, (unsigned)wgs, FastDiv::make((unsigned)(cols ? tiles_n : units))};
@@ -116,7 +117,7 @@ int psgdk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int
     if (rows == 0 || cols == 0) return PSGDK_OK;
     if (!codes || !scales || !out || !mx_aligned(codes, 16) || !mx_aligned(out, mx_size(out_dtype))) return PSGDK_ERR_INVALID;
     const int64_t units = mx_pad(cols) / MX_PAD, need = (rows * units + 7) / 8;
-    if (need > (1ll << 28)) return PSGDK_ERR_UNSUPPORTED;
+    if (need > kMaxThreads / 256) return PSGDK_ERR_UNSUPPORTED;
     const FastDiv div = FastDiv::make((unsigned)units);
     const hipStream_t st = (hipStream_t)stream;
     return mx_by_dtype(out_dtype, [&](auto* e) {
@@ -141,7 +142,7 @@ int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int
         !mx_aligned(codes, 16) || !mx_aligned(codes_t, 16)) return PSGDK_ERR_INVALID;
     const hipStream_t st = (hipStream_t)stream;
     const int64_t tiles_n = (cols + 127) / 128, tiles = mx_pad(rows) / 128 * tiles_n;
-    if (codes_t && tiles > (1ll << 28)) return PSGDK_ERR_UNSUPPORTED;
+    if ((cols <= 2048 ? (rows + 3) / 4 : rows) > kMaxThreads / 256 || (codes_t && tiles > kMaxThreads / (128 * size))) return PSGDK_ERR_UNSUPPORTED;
     return mx_by_dtype(dtype, [&](auto* e) {
         using T = std::remove_pointer_t<decltype(e)>;
 #define MX_NORM(F) mx_norm_by_cols<T, F>((int)cols, x, residual, gain, gain_dtype, s, inv, (uint8_t*)codes, (uint8_t*)scales, (int)rows, (int)cols, eps, st)

@@ -90,7 +90,7 @@ int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_
     const size_t need = p.splits > 1 ? (size_t)p.splits * m * n * 4 : 0;
     if (need && (!work || work_bytes < need || !mx_aligned(work, 16))) return PSGDK_ERR_INVALID;
     const int64_t tm = p.skinny ? 1 : (m + p.bm - 1) / p.bm, tn = p.skinny ? 1 : (n + p.bn - 1) / p.bn;
-    if (tm * tn * p.splits > (1ll << 28) || (need && m * n / 1024 > (1ll << 28))) return PSGDK_ERR_UNSUPPORTED;
+    if (tm * tn * p.splits > kMaxThreads / 256 || (need && (m * n + 1023) / 1024 > kMaxThreads / 256)) return PSGDK_ERR_UNSUPPORTED;
     const MxGemm g{(const uint8_t*)a_codes, (const uint8_t*)a_scales, (const uint8_t*)b_codes, (const uint8_t*)b_scales, out, need ? (float*)work : nullptr, n,
                    (int)m, (int)n, (int)KS, out_dtype, p.splits, (int)tm, (int)tn};
     const hipStream_t st = (hipStream_t)stream;

@@ -227,3 +227,17 @@ def test_copies_and_pickles_have_addresses_of_their_own():
             assert c._ptrs == (c.codes.data_ptr(), c.scales.data_ptr()) and not set(c._ptrs) & set(t._ptrs)
         c = copy.copy(t)                                     # the same memory, held by the copy too
         assert c._ptrs == t._ptrs == (c.codes.data_ptr(), c.scales.data_ptr())
+
+
+def test_more_threads_than_a_launch_can_have_are_refused(lib):
+    # (2^32 threads; addresses are never reached)
+    t = _arg(rows=1 << 28)
+    assert lib.psgdk_mx_quantize(1, C.byref(t), 0, 4, None) == 2
+    t = _arg(rows=1 << 30, cols=128 * 8, ld=1 << 10, codes=None, scales=None, codes_t=8192, scales_t=8192)
+    assert lib.psgdk_mx_quantize(1, C.byref(t), 1, 4, None) == 2
+    assert lib.psgdk_mx_dequantize(4096, 4096, 1 << 28, 64, 4, 8192, 0, None) == 2
+    ok = [4096, None, 4096, 1, 1 << 27, 64, 0, 1e-5, 8, None, 8192, 8192, 8192, None, None, None]
+    assert lib.psgdk_rms_norm_mx(*ok) == 2
+    ok[4], ok[5] = 1 << 25, 4096
+    assert lib.psgdk_rms_norm_mx(*ok) == 2
+    assert lib.psgdk_mx_matmul(4096, 4096, 1 << 30, 4, 4096, 4096, 1 << 12, 4, 256, 8192, 0, 65536, 1 << 60, None) == 2
