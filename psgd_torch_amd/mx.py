@@ -162,6 +162,22 @@ class MxTensor:
         """The tensors that hold it (autograd saves these, and sees by them whether it was written again)."""
         return [self._codes, self._scales] if self._buffer is None else [self._buffer]
 
+    def _form(self):
+        """What _of needs besides the memory."""
+        return self.shape, self.fmt, self._at, 2 if self._buffer is None else 1
+
+    @classmethod
+    def _of(cls, form, memory) -> "MxTensor":
+        """The matrix that had this _form(), in the tensors that its _memory() has become."""
+        shape, fmt, at, n = form
+        if n == 2:
+            return cls(*memory, shape, fmt)
+        t = object.__new__(cls)
+        t._buffer, = memory
+        base = t._buffer.data_ptr()
+        t.shape, t.fmt, t.device, t._codes, t._scales, t._at, t._ptrs = shape, fmt, t._buffer.device, None, None, at, (base, base + at)
+        return t
+
     def dequantize(self, dtype=torch.bfloat16) -> torch.Tensor:
         return mx_dequantize(self, dtype)
 
@@ -417,20 +433,31 @@ def _tracked(*ts):
     return ts if torch.is_grad_enabled() else tuple(None if t is None else t.detach() for t in ts)
 
 
-def _product_grads(ctx, dout, need_x, need_w, x_dtype):
-    """(gradient of the product's input in x_dtype, of the weight) from dout."""
+def _product_grads(ctx, saved, dout, need_x, need_w, x_dtype):
+    """(gradient of the product's input in x_dtype, of the weight) from dout; saved: what _keep saved behind `more`."""
     dr, dc = _rounded(_rows("gradient", dout), ctx.grad_fmt, need_x, need_w)
-    dx = _matmul(dr, ctx.cols, x_dtype, _DTYPE[x_dtype]) if need_x else None
-    dw = _matmul(dc, ctx.act, ctx.weight_dtype, _DTYPE[ctx.weight_dtype]) if need_w else None
+    dx = dw = None
+    if need_x:
+        n = ctx.cols[3]
+        dx = _matmul(dr, MxTensor._of(ctx.cols, saved[:n]), x_dtype, _DTYPE[x_dtype])
+        saved = saved[n:]
+    if need_w:
+        dw = _matmul(dc, MxTensor._of(ctx.act, saved), ctx.weight_dtype, _DTYPE[ctx.weight_dtype])
     return dx, dw
 
 
 def _keep(ctx, weight, param, act, need_x, need_w, grad_fmt, *more):
-    """What the backward pass needs: the MX forms on ctx, the memory they lie in saved, so that autograd refuses what was written again."""
-    ctx.cols, ctx.act = weight.cols if need_x else None, act if need_w else None
+    """What the backward pass needs.  The memory of the MX forms is saved as tensors and ctx holds no form itself: autograd refuses what was written
+    again, frees the activations once they are used, and hands them to whoever packs saved tensors (checkpoints, offloading)."""
+    memory = []
     if need_x:
         _need_cols(weight)
-    ctx.save_for_backward(*more, *(weight.cols._memory() if need_x else ()), *(act._memory() if need_w else ()))
+        ctx.cols = weight.cols._form()
+        memory += weight.cols._memory()
+    if need_w:
+        ctx.act = act._form()
+        memory += act._memory()
+    ctx.save_for_backward(*more, *memory)
     ctx.weight_dtype, ctx.grad_fmt = param.dtype, grad_fmt
 
 
@@ -448,8 +475,7 @@ class _Linear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         need_x, need_w = ctx.needs_input_grad[:2]
-        ctx.saved_tensors                                # (raises where a kept form was renewed since)
-        dx, dw = _product_grads(ctx, dout, need_x, need_w, ctx.x_dtype)
+        dx, dw = _product_grads(ctx, ctx.saved_tensors, dout, need_x, need_w, ctx.x_dtype)      # (raises where a kept form was renewed since)
         return (dx.view(ctx.x_shape) if need_x else None), dw, None, None, None
 
 
@@ -462,6 +488,8 @@ class _NormLinear(torch.autograd.Function):
         out = _matmul(yr, weight.rows, x.dtype, _DTYPE[x.dtype])
         _keep(ctx, weight, param, yc, need_s or need_g, need_w, grad_fmt, s, inv, gain)
         ctx.set_materialize_grads(False)
+        if residual is not None and not need_s:
+            ctx.mark_non_differentiable(s)
         out = out if x.dim() == 2 else out.view(*x.shape[:-1], weight.rows.shape[0])
         return out if residual is None else (out, s)
 
@@ -471,11 +499,11 @@ class _NormLinear(torch.autograd.Function):
         need_s = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         need_g, need_w = ctx.needs_input_grad[2:4]
         need_y = need_s or need_g
-        s, inv, gain = ctx.saved_tensors[:3]
+        s, inv, gain, *saved = ctx.saved_tensors
         dx = dg = dw = None
         if dout is not None:
             # (the gradient of y stays in fp32 between the two kernels: one rounding, at dx)
-            dy, dw = _product_grads(ctx, dout, need_y, need_w, torch.float32)
+            dy, dw = _product_grads(ctx, saved, dout, need_y, need_w, torch.float32)
             if need_y:
                 dx, dg = _norm_backward(dy.view(s.shape), s, gain, inv, ds)
                 dg = dg.to(gain.dtype)

@@ -689,3 +689,76 @@ def test_offsets_past_32_bits(p):
     assert bool(((big[-130:] - small).abs() <= 1e-5 * small.abs().max()).all())
     big = p.mx_matmul(w, q, out_dtype=torch.float32)                            # the long operand second, few rows first
     assert bool(((big[:, -130:] - small.t()).abs() <= 1e-5 * small.abs().max()).all())
+
+
+def _layers(p, seed, t=300, k=512, n=520):
+    g = torch.Generator().manual_seed(seed)
+    x, res = (torch.randn(t, k, generator=g).to(DEV, torch.bfloat16).requires_grad_() for _ in range(2))
+    gain = (1 + 0.1 * torch.randn(k, generator=g)).to(DEV).requires_grad_()
+    w, v = (p.MxWeight(torch.nn.Parameter(0.05 * torch.randn(*s, generator=g).to(DEV)), "fp4") for s in ((n, k), (k, n)))
+
+    def run(x, res, gain):
+        y, s = p.mx_norm_linear(x, gain, w, res)
+        return p.mx_linear(y, v) + s
+    return run, (x, res, gain), (w, v)
+
+
+def test_activations_are_freed_by_the_backward_pass(p):
+    run, leaves, ws = _layers(p, 50, t=4096)
+    grads = lambda out: torch.autograd.grad(out.float().square().sum(), (*leaves, *(w.param for w in ws)))      # noqa: E731
+    grads(run(*leaves))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    out = run(*leaves)
+    held = torch.cuda.memory_allocated() - before
+    got = grads(out)
+    del got
+    left = torch.cuda.memory_allocated() - before
+    # held: the output, s, the activations of both layers (fp8, 1 byte an element and more); left, with the graph's nodes alive: the output, in 2 bytes
+    assert out.grad_fn is not None and held > left and left <= 2 * out.numel() + 4096, (held, left)
+    with pytest.raises(RuntimeError):
+        grads(out)
+
+
+@pytest.mark.parametrize("way", ["checkpoint", "offload"])
+def test_saved_tensors_may_be_packed(p, way):
+    from torch.utils.checkpoint import checkpoint
+    run, leaves, ws = _layers(p, 51)
+    wrt = (*leaves, *(w.param for w in ws))
+    want = torch.autograd.grad(run(*leaves).float().square().sum(), wrt)
+    if way == "checkpoint":
+        got = torch.autograd.grad(checkpoint(run, *leaves, use_reentrant=False).float().square().sum(), wrt)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            out = run(*leaves)
+        for w in ws:                                                   # (what was packed is what counts)
+            with torch.no_grad():
+                w.param.mul_(2)
+            w.refresh()
+        got = torch.autograd.grad(out.float().square().sum(), wrt)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_s_needs_a_gradient_only_through_its_terms(p):
+    run, (x, res, gain), (w, _) = _layers(p, 52)
+    y, s = p.mx_norm_linear(x.detach(), gain, w, res.detach())
+    assert y.requires_grad and not s.requires_grad
+    y.float().sum().backward()
+    assert gain.grad is not None and w.param.grad is not None
+    y, s = p.mx_norm_linear(x.detach(), gain, w, res)
+    assert y.requires_grad and s.requires_grad
+
+
+def test_layers_under_a_deep_copied_module(p):
+    import copy
+    run, leaves, (w, _) = _layers(p, 53)
+    x = leaves[0].detach()
+    want = p.mx_linear(x, w).detach()
+    c = copy.deepcopy(w)
+    with torch.no_grad():
+        w.param.zero_()
+    w.refresh()
+    assert torch.equal(p.mx_linear(x, c), want) and not p.mx_linear(x, w).any()
+    c.refresh()
+    assert torch.equal(p.mx_linear(x, c), want)
