@@ -385,7 +385,8 @@ int psgdk_profile_read_calls(psgdk_plan* plan, double* call_ms, int64_t* calls, 
  * block of zeros; a block that holds an infinity or a NaN has the byte 255 and reads as NaN.  A rows x cols matrix is stored row by row, blocks
  * along its rows, a row's codes in multiples of 256 elements (zeros behind the last), its scales in multiples of 8 bytes: psgdk_mx_storage.  The
  * calls below read and write whole stored rows.  Codes and `work` are aligned to 16 bytes, scales to 8.  All calls are stream-ordered, allocate
- * nothing, keep nothing and may be captured into a graph. */
+ * nothing, keep nothing and may be captured into a graph.  What would need 2^32 threads in a launch (2^24 rows at the least) or passes a limit
+ * below returns PSGDK_ERR_UNSUPPORTED. */
 enum { PSGDK_MX_FP4 = 4, PSGDK_MX_FP8 = 8 };
 #define PSGDK_NORM_MAX_COLS 16384
 
@@ -410,7 +411,8 @@ int psgdk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int
 int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int out_dtype, size_t* bytes);
 int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_fmt, const void* b_codes, const void* b_scales, int64_t n, int b_fmt,
                     int64_t k, void* out, int out_dtype, void* work, size_t work_bytes, void* stream);
-/* s = x + residual, rounded to dtype (residual NULL: s is x, nothing is written); inv = (mean of s^2 + eps)^-1/2 of every row; y = s inv gain in MX
+/* s = x + residual, rounded to dtype (residual NULL: s is x, nothing is written); inv = (mean of s^2 + eps)^-1/2 of every row, squares and sum in
+ * fp32 (a row whose sum of squares passes fp32's range has inv 0); y = s inv gain in MX
  * form (codes), and y transposed in MX form (codes_t); either may be NULL.  cols <= PSGDK_NORM_MAX_COLS.  s may be x or residual. */
 int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int gain_dtype, int64_t rows, int64_t cols, int dtype, float eps, int fmt,
                       void* s, float* inv, void* codes, void* scales, void* codes_t, void* scales_t, void* stream);
