@@ -22,7 +22,7 @@ template <typename T, int FMT, int THREADS, int CH>
 static void mx_norm_one(const void* x, const void* res, const void* gain, int gdt, void* s, float* inv, uint8_t* codes, uint8_t* scales, int rows,
                         int cols, float eps, hipStream_t st) {
     const unsigned grid = THREADS == 64 ? (rows + 3) / 4 : rows;
-    rms_norm_mx_kernel<T, FMT, THREADS, CH><<<grid, 256, 0, st>>>((const T*)x, (const T*)res, gain, gdt, (T*)s, inv, codes, scales, rows, cols, eps);
+    rms_norm_mx_kernel<T, FMT, THREADS, CH><<<grid, 256, 0, st>>>((const T*)x, (const T*)res, gain, gdt, (T*)s, inv, codes, scales, rows, cols, 1.0 / cols, eps);
 }
 // one wave a row up to 2048 columns, a workgroup a row up to 16384
 template <typename T, int FMT, typename... A>
