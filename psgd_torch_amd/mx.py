@@ -293,9 +293,9 @@ def _norm_args(x, gain, residual):
 def rms_norm_mx(x: torch.Tensor, gain: torch.Tensor, residual: Optional[torch.Tensor] = None, *, eps: float = 1e-5, fmt: str = "fp8",
                 which: str = "rows"):
     """s = x + residual (rounded to x's dtype; without a residual s is x), inv = (mean of s^2 + eps)^-1/2 of every row in fp32, y = s inv gain.
-    Returns (y in MX form as mx_quantize's `which` says, s, inv).  y is rounded once, from fp32; a row whose sum of squares passes fp32's range has
-    inv 0.  At most 16384 columns.  Not differentiable by
-    itself (rms_norm_mx_backward has the gradients, mx_norm_linear is the differentiable layer)."""
+    Returns (y in MX form as mx_quantize's `which` says, s, inv).  The squares are summed in 64 bits, inv is the fp32 number nearest to the exact one, y is
+    rounded once, from fp32.  At most 16384 columns.  Not differentiable by itself (rms_norm_mx_backward has the gradients, mx_norm_linear is the
+    differentiable layer)."""
     _norm_args(x, gain, residual)
     if torch.is_grad_enabled() and (x.requires_grad or gain.requires_grad or residual is not None and residual.requires_grad):
         raise _bad("rms_norm_mx does not record gradients: use mx_norm_linear, or call it under torch.no_grad()")

@@ -762,3 +762,35 @@ def test_layers_under_a_deep_copied_module(p):
     assert torch.equal(p.mx_linear(x, c), want) and not p.mx_linear(x, w).any()
     c.refresh()
     assert torch.equal(p.mx_linear(x, c), want)
+
+
+# ---- the norm's sums ---------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,cols", [(2049, 520), (1500, 768), (700, 2100), (300, 4096), (70, 16384)])
+@pytest.mark.parametrize("dt", DTYPES)
+def test_norm_inv_is_the_nearest(p, rows, cols, dt):
+    """Squares and their sum are held in 64 bits: inv is off by its own rounding alone, half a step of fp32 (and 2^-40, far above what 16384 additions in 64
+    bits can amount to).  y is then off by inv's rounding and its own, in either form, whatever the number of rows."""
+    g = torch.Generator().manual_seed(61)
+    x, r = (torch.randn(rows, cols, generator=g).to(dt) for _ in range(2))
+    gain = 1 + 0.3 * torch.randn(cols, generator=g)
+    s, inv, y = O.norm(x, gain, r, 1e-5)
+    (yr, yc), gs, ginv = p.rms_norm_mx(x.to(DEV), gain.to(DEV), r.to(DEV), which="both")
+    assert torch.equal(gs.cpu(), s)
+    assert bool(((ginv.cpu().double() - inv).abs() <= (EPS24 + 2.0 ** -40) * inv).all())
+    _check_norm_codes(yr, y, "fp8", cols, 2.01 * EPS24)
+    _check_norm_codes(yc, y.t().contiguous(), "fp8", rows, 2.01 * EPS24)
+
+
+def test_norm_of_very_large_and_very_small_rows(p):
+    """Sums of squares far outside fp32's range: the rows are normalised like any other."""
+    g = torch.Generator().manual_seed(62)
+    x = torch.randn(6, 700, generator=g) * torch.tensor([1e25, 1e-25, 1.0, 1e36, 1e-30, 1e19])[:, None]
+    gain = torch.ones(700)
+    for dt in (torch.float32, torch.bfloat16):
+        s, inv, y = O.norm(x.to(dt), gain, None, 0.0)
+        (yr, yc), _, ginv = p.rms_norm_mx(x.to(dt).to(DEV), gain.to(DEV), eps=0.0, which="both")
+        # (the smallest number here, 1e-36, is normal)
+        assert bool(((ginv.cpu().double() - inv).abs() <= (EPS24 + 2.0 ** -40) * inv).all())
+        _check_norm_codes(yr, y, "fp8", 700, 2.01 * EPS24)
+        _check_norm_codes(yc, y.t().contiguous(), "fp8", 6, 2.01 * EPS24)
