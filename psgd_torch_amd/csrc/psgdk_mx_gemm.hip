@@ -1,5 +1,6 @@
 // psgdk_mx_gemm.hip -- psgdk_mx_matmul (include/psgdk.h, "microscaled numbers"): argument checks, choice of kernel, launches.
 #include <cmath>
+#include "../../include/psgdk_test.h"
 #include "mx_host.hiph"
 #include "gemm_mx.hiph"
 
@@ -101,6 +102,17 @@ int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_
     }
     if (a_fmt == PSGDK_MX_FP4) return mx_launch_product<4, 8, false>(g, p, st);
     return b_fmt == PSGDK_MX_FP4 ? mx_launch_product<8, 4, false>(g, p, st) : mx_launch_product<8, 8, false>(g, p, st);
+}
+
+int psgdk_test_mx_plan(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int out_dtype, int* rows, int* cols, int* splits, int* wide) {
+    if (m < 1 || n < 1 || k < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim || !rows || !cols || !splits || !wide) return PSGDK_ERR_INVALID;
+    if (!mx_fmt_ok(a_fmt) || !mx_fmt_ok(b_fmt) || !mx_dtype_ok(out_dtype)) return PSGDK_ERR_INVALID;
+    *wide = mx_wide(a_fmt, b_fmt, out_dtype);
+    const MxPlan p = mx_plan(m, n, mx_pad(k) / MX_PAD, a_fmt, b_fmt, *wide);
+    *rows = p.skinny ? 16 * p.mt : p.bm;
+    *cols = p.skinny ? 0 : p.bn;
+    *splits = p.skinny ? p.kw : p.splits;
+    return PSGDK_OK;
 }
 
 }  // extern "C"

@@ -794,3 +794,77 @@ def test_norm_of_very_large_and_very_small_rows(p):
         assert bool(((ginv.cpu().double() - inv).abs() <= (EPS24 + 2.0 ** -40) * inv).all())
         _check_norm_codes(yr, y, "fp8", 700, 2.01 * EPS24)
         _check_norm_codes(yc, y.t().contiguous(), "fp8", 6, 2.01 * EPS24)
+
+
+# ---- products, kernel by kernel ----------------------------------------------------------------------------------------------------------
+
+FMT = {"fp4": 4, "fp8": 8}
+PAIRS = [("fp4", "fp4"), ("fp4", "fp8"), ("fp8", "fp4"), ("fp8", "fp8")]
+
+
+def _plan(p, m, n, k, fa, fb, dt):
+    """(tile rows, tile columns, splits of K, WIDE) that the library chooses; 0 columns: the few-rows kernel."""
+    import ctypes as C
+    from psgd_torch_amd import _lib
+    out = [C.c_int() for _ in range(4)]
+    assert _lib.lib().psgdk_test_mx_plan(m, n, k, FMT[fa], FMT[fb], p.mx._DTYPE[dt], *[C.byref(v) for v in out]) == 0
+    return tuple(v.value for v in out)
+
+
+def _device_operand(p, rows, k, fmt, seed, scales=None):
+    """(MX form, its values in 64 bits on the device) of normally distributed numbers; scales: a factor for each block of 32 (rows x blocks)."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(rows, k, generator=g, device=DEV)
+    if scales is not None:
+        x = x * scales.to(DEV).repeat_interleave(32, 1)[:, :k]
+    q = p.mx_quantize(x, fmt)
+    return q, p.mx_dequantize(q, torch.float32).double()
+
+
+def _product_into_guarded(p, qa, qb, dt):
+    """mx_matmul by the C call into the middle of a larger buffer: what lies before and behind the output stays as it was."""
+    import ctypes as C
+    from psgd_torch_amd import _lib
+    (m, k), n, lib, code = qa.shape, qb.shape[0], _lib.lib(), p.mx._DTYPE[dt]
+    guard = 1 << 16
+    buf = torch.full((m * n + 2 * guard,), 77.0, dtype=dt, device=DEV)
+    out = buf[guard:guard + m * n].view(m, n)
+    wb = C.c_size_t()
+    assert lib.psgdk_mx_matmul_work_bytes(m, n, k, FMT[qa.fmt], FMT[qb.fmt], code, C.byref(wb)) == 0
+    work = torch.empty(max(wb.value, 16), dtype=torch.uint8, device=DEV)
+    rc = lib.psgdk_mx_matmul(*qa._ptrs, m, FMT[qa.fmt], *qb._ptrs, n, FMT[qb.fmt], k, out.data_ptr(), code, work.data_ptr(), wb.value,
+                             torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert bool((buf[:guard] == 77).all()) and bool((buf[guard + m * n:] == 77).all())
+    return out
+
+
+def _check_kernel(p, m, n, k, fa, fb, dt, tile, splits=None):
+    plan = _plan(p, m, n, k, fa, fb, dt)
+    assert plan[:2] == tile and (splits is None or plan[2] == splits), (m, n, k, fa, fb, dt, plan)
+    (qa, a), (qb, b) = _device_operand(p, m, k, fa, 71), _device_operand(p, n, k, fb, 72)
+    want = a @ b.t().contiguous()
+    got = _product_into_guarded(p, qa, qb, dt)
+    _check_product(got, a, b, want, "fp8" in (fa, fb) and dt != torch.float32)
+    assert torch.equal(p.mx_matmul(qa, qb, out_dtype=dt), got)                    # the same bits, whatever lies around the output
+    # the first rows by themselves, through the few-rows kernel
+    few = p.MxTensor(qa.codes[:3], qa.scales[:3], (3, k), fa)
+    assert _plan(p, 3, n, k, fa, fb, dt)[1] == 0
+    _check_product(p.mx_matmul(few, qb, out_dtype=dt), a[:3], b, want[:3], "fp8" in (fa, fb) and dt != torch.float32)
+
+
+# ragged in M and N (an odd output pitch, the last tile's columns stored one by one), K past a multiple of 256: 3, 5, 9 and 10 blocks, of which scales come in fours
+LARGE = [(4090, 4095, 2500, fa, fb, dt) for fa, fb in PAIRS for dt in (torch.bfloat16, torch.float16)] + \
+        [(4090, 4095, 2500, "fp4", "fp4", torch.float32)] + \
+        [(3900, 4091, 2049, fa, fb, torch.bfloat16) for fa, fb in PAIRS] + [(4090, 4095, 700, fa, fb, torch.bfloat16) for fa, fb in PAIRS[1:]] + \
+        [(4095, 4090, 1300, fa, fb, torch.bfloat16) for fa, fb in PAIRS[1:]]
+
+
+@pytest.mark.parametrize("m,n,k,fa,fb,dt", LARGE)
+def test_matmul_tiles_of_256(p, m, n, k, fa, fb, dt):
+    _check_kernel(p, m, n, k, fa, fb, dt, (256, 256), 1)
+
+
+@pytest.mark.parametrize("fa,fb", PAIRS[1:])
+def test_matmul_tiles_of_256_split(p, fa, fb):
+    _check_kernel(p, 4345, 139, 33900, fa, fb, torch.bfloat16, (256, 256), 8)

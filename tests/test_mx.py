@@ -241,3 +241,16 @@ def test_more_threads_than_a_launch_can_have_are_refused(lib):
     ok[4], ok[5] = 1 << 25, 4096
     assert lib.psgdk_rms_norm_mx(*ok) == 2
     assert lib.psgdk_mx_matmul(4096, 4096, 1 << 30, 4, 4096, 4096, 1 << 12, 4, 256, 8192, 0, 65536, 1 << 60, None) == 2
+
+
+def test_plan_query(lib):
+    """psgdk_test_mx_plan: which kernel a product takes, and its refusals."""
+    def plan(*a):
+        out = [C.c_int(-1) for _ in range(4)]
+        return lib.psgdk_test_mx_plan(*a, *[C.byref(v) for v in out]), tuple(v.value for v in out)
+    assert plan(3, 1000, 512, 4, 8, 0) == (0, (16, 0, 2, 0)) and plan(33, 100, 512, 8, 8, 1) == (0, (48, 0, 2, 1))
+    assert plan(8192, 8192, 8192, 4, 4, 0) == (0, (256, 256, 1, 0)) and plan(300, 300, 300, 8, 4, 1) == (0, (128, 128, 1, 1))
+    assert plan(50, 16500, 600, 8, 4, 0) == (0, (64, 128, 1, 0))
+    for bad in ((0, 1, 1, 4, 4, 0), (1, 0, 1, 4, 4, 0), (1, 1, -1, 4, 4, 0), (1, 1, 1, 5, 4, 0), (1, 1, 1, 4, 5, 0), (1, 1, 1, 4, 4, 3), (1 << 31, 1, 1, 4, 4, 0)):
+        assert plan(*bad)[0] == 1
+    assert lib.psgdk_test_mx_plan(1, 1, 1, 4, 4, 0, None, None, None, None) == 1
