@@ -868,3 +868,11 @@ def test_matmul_tiles_of_256(p, m, n, k, fa, fb, dt):
 @pytest.mark.parametrize("fa,fb", PAIRS[1:])
 def test_matmul_tiles_of_256_split(p, fa, fb):
     _check_kernel(p, 4345, 139, 33900, fa, fb, torch.bfloat16, (256, 256), 8)
+
+
+@pytest.mark.parametrize("fa,fb", PAIRS)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k,splits", [(33, 50001, 200, 1), (50, 16500, 600, 1), (5, 50257, 1100, 1), (64, 33001, 513, 1), (17, 40001, 520, 1), (64, 4099, 4000, None),
+                                          (33, 2001, 5900, 8)])
+def test_matmul_tiles_of_64(p, m, n, k, splits, fa, fb, dt):
+    _check_kernel(p, m, n, k, fa, fb, dt, (64, 128), splits)
