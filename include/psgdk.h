@@ -404,9 +404,9 @@ int psgdk_mx_storage(int64_t rows, int64_t cols, int fmt, int64_t* code_bytes, i
 int psgdk_mx_quantize(int count, const psgdk_mx_tensor* tensors, int dtype, int fmt, void* stream);
 /* out (rows x cols, packed) = the values codes and scales stand for */
 int psgdk_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t cols, int fmt, void* out, int out_dtype, void* stream);
-/* out (m x n, packed) = A B^T of A (m x k) and B (n x k), either in either format, n <= 2^22 and k <= 2^23; fp32 sums, rounded once.  With an 8-bit operand the matrix
- * instruction drops the bits of a product below 2^-13 of the largest one it adds: taken for 16-bit outputs.  An fp32 output
- * has fp32 sums throughout (at half the rate; elements below 2^-126 count as zero there).  `work`: psgdk_mx_matmul_work_bytes
+/* out (m x n, packed) = A B^T of A (m x k) and B (n x k), either in either format, n <= 2^22 and k <= 2^23; fp32 sums, rounded once.  With an 8-bit operand and a
+ * 16-bit output the matrix instruction drops the bits of a product below 2^-13 of the largest one in its block of 32.  An fp32 output has fp32 sums
+ * throughout (with an 8-bit operand at half the rate; elements below 2^-126 count as zero there).  `work`: psgdk_mx_matmul_work_bytes
  * (0 where the contraction is not split), free for other use once the call's kernels have run. */
 int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int out_dtype, size_t* bytes);
 int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_fmt, const void* b_codes, const void* b_scales, int64_t n, int b_fmt,

@@ -251,9 +251,10 @@ def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
 def mx_matmul(a: MxTensor, b: MxTensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """A B^T (M x N) of a (M x K) and b (N x K), either in either format; fp32 sums, rounded once to out_dtype.  The same inputs give the same bits:
     a long contraction with few outputs is split, and the parts are added in a fixed order.
-    With an fp8 operand the scaled matrix instruction drops the bits of a product below 2^-13 of the largest one it adds (about 2e-5 of a result):
-    that is taken for 16-bit outputs, whose own rounding is a hundred times larger.  An fp32 output has fp32 sums throughout, at half the rate
-    (elements below 2^-126 count as zero there)."""
+    With an fp8 operand and a 16-bit output the scaled matrix instruction drops the bits of a product below 2^-13 of the largest one in its block of 32.
+    For normally distributed operands that is 2e-5 of the results, a hundredth of a bf16 output's rounding; where the large products of a block cancel, what
+    is left may be off by up to 32 2^-13 of the largest.  An fp32 output has fp32 sums throughout: at half the rate with an fp8 operand (elements
+    below 2^-126 count as zero there), at the full rate with two fp4 operands."""
     _mx("a", a)
     _mx("b", b, a.device)
     if a.shape[1] != b.shape[1]:

@@ -876,3 +876,67 @@ def test_matmul_tiles_of_256_split(p, fa, fb):
                                           (33, 2001, 5900, 8)])
 def test_matmul_tiles_of_64(p, m, n, k, splits, fa, fb, dt):
     _check_kernel(p, m, n, k, fa, fb, dt, (64, 128), splits)
+
+
+def _block_maxima(a, b):
+    """The sum over K's blocks of 32 of the largest product of each, for every element of A B^T (M x N, 64 bits)."""
+    k = -(-a.shape[1] // 32) * 32
+    a, b = (torch.nn.functional.pad(v.abs(), (0, k - v.shape[1])) for v in (a, b))
+    out = torch.zeros(a.shape[0], b.shape[0], dtype=torch.float64, device=a.device)
+    for i in range(0, k, 32):
+        out += (a[:, None, i:i + 32] * b[None, :, i:i + 32]).amax(-1)
+    return out
+
+
+@pytest.mark.parametrize("spread", [2, 8, 13, 20, 30])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 128), (3, 40, 1000), (50, 300, 1000), (300, 300, 1024)])
+@pytest.mark.parametrize("fa,fb", PAIRS)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_matmul_of_blocks_far_apart(p, m, n, k, fa, fb, dt, spread):
+    """Scales within a row up to 2^spread apart on either side.  Sums are fp32 sums of the blocks (_product_bound); an 8-bit operand and a 16-bit output
+    add what the scaled instruction drops: of each of a block's 32 products less than 2^-13 of the largest one of that block."""
+    g = torch.Generator().manual_seed(73)
+    sa, sb = (torch.exp2((torch.rand(r, -(-k // 32), generator=g) * (spread + 1)).floor()) for r in (m, n))
+    (qa, a), (qb, b) = _device_operand(p, m, k, fa, 74, sa), _device_operand(p, n, k, fb, 75, sb * 2.0 ** -spread)
+    want = a @ b.t().contiguous()
+    if dt == torch.float16:
+        (qa, a), (qb, b) = _device_operand(p, m, k, fa, 74, sa * 2.0 ** -spread), _device_operand(p, n, k, fb, 75, sb * 2.0 ** -spread)
+        want = a @ b.t().contiguous()
+        assert float(want.abs().max()) < 60000
+    got = p.mx_matmul(qa, qb, out_dtype=dt)
+    bound = _product_bound(a, b, dt, want, False)
+    if "fp8" in (fa, fb) and dt != torch.float32:
+        bound = bound + 32 * 2.0 ** -13 * _block_maxima(a, b)
+    err = (got.double() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+def test_matmul_sums_of_two_4_bit_operands_are_fp32_sums(p):
+    """What one instruction adds (128 elements) with two 4-bit operands: a large pair that cancels within its block leaves a later block's small product as
+    it is, whatever its size; where the small one has to share a partial sum with a large one, it is kept while 2^gap + 1 has 24 bits (an fp32 sum can
+    promise no more, in whatever order it adds)."""
+    for gap in range(0, 45):
+        for i, j, l, most in ((0, 1, 32, 99), (3, 31, 96, 99), (64, 70, 0, 23), (0, 64, 32, 23), (32, 96, 64, 23)):
+            x = torch.zeros(2, 128)
+            x[:, i], x[:, j], x[:, l] = 2.0 ** gap, -2.0 ** gap, 1.0
+            a, b = p.mx_quantize(x.to(DEV)), p.mx_quantize(torch.ones(20, 128, device=DEV))
+            assert torch.equal(p.mx_dequantize(a, torch.float32).cpu(), x)
+            got = p.mx_matmul(a, b, out_dtype=torch.float32).cpu()
+            if gap <= most:
+                assert torch.equal(got, torch.ones(2, 20)), (gap, i, j, l)
+            else:
+                assert bool(((got == 0) | (got == 1)).all()), (gap, i, j, l)
+
+
+def test_matmul_bits_dropped_with_an_8_bit_operand(p):
+    """One large product, its negative in the next 128 elements, a small one beside the first: with a 16-bit output what lies below 2^-13 of the largest of
+    the block is dropped, with a 32-bit output nothing is."""
+    for fa, fb in PAIRS[1:]:
+        for e in range(8, -10, -1):
+            x = torch.zeros(1, 256)
+            x[0, 0], x[0, 3], x[0, 128] = 256.0, 2.0 ** e, -256.0
+            one = torch.ones(20, 256)
+            a, b = (p.mx_quantize(v.to(DEV), f) for v, f in (((x, fa), (one, fb)) if fa == "fp8" else ((one[:1], fa), (x.expand(20, 256), fb))))
+            assert bool((p.mx_matmul(a, b, out_dtype=torch.float32) == 2.0 ** e).all())
+            got = p.mx_matmul(a, b)
+            assert bool(((got.float() - 2.0 ** e).abs() <= 256 * 2.0 ** -13).all())
