@@ -365,7 +365,8 @@ def _norm_backward(dy, s, gain, inv, ds):
 class MxWeight:
     """The MX forms of a 2-D parameter (N x K): `rows` (blocks along K: the forward product) and `cols` (the transpose, blocks along N: the gradient of
     the layer's input).  They are rounded once here and renewed by refresh() -- KWNS4.keep_mx does that after every step.  `rows` / `cols` may be
-    handed over instead; backward=False keeps the forward form only."""
+    handed over instead: such a form keeps its contents until the first refresh, and only what is missing is rounded here.  backward=False keeps the
+    forward form only (and `cols` where it is handed over)."""
 
     def __init__(self, param: torch.Tensor, fmt: str = "fp4", *, backward: bool = True, rows: Optional[MxTensor] = None, cols: Optional[MxTensor] = None):
         _tensor("param", param)
@@ -378,16 +379,16 @@ class MxWeight:
         for what, t, shape in (("rows", rows, (n, k)), ("cols", cols, (k, n))):
             if t is not None and _mx(what, t, param.device).shape != shape:
                 raise _bad(f"MxWeight {what} is {t.shape[0]} x {t.shape[1]}, expected {shape[0]} x {shape[1]}")
+        _fmt(fmt)
+        if rows is not None and cols is not None and cols.fmt != rows.fmt:
+            raise _bad(f"MxWeight rows are {rows.fmt}, cols {cols.fmt}")
         self.param = param
-        self.fmt = rows.fmt if rows is not None else fmt
-        _fmt(self.fmt)
-        if cols is not None and cols.fmt != self.fmt:
-            raise _bad(f"MxWeight rows are {self.fmt}, cols {cols.fmt}")
-        given = rows is not None
-        self.rows = rows if given else MxTensor.empty(n, k, self.fmt, param.device)
-        self.cols = cols if cols is not None else MxTensor.empty(k, n, self.fmt, param.device) if backward and not given else None
-        if not given:
-            self.refresh()
+        self.fmt = rows.fmt if rows is not None else cols.fmt if cols is not None else fmt
+        need_rows, need_cols = rows is None, cols is None and backward
+        if need_rows or need_cols:
+            r, c = _rounded(_rows("param", param.detach()), self.fmt, need_rows, need_cols)
+            rows, cols = rows if rows is not None else r, cols if cols is not None else c
+        self.rows, self.cols = rows, cols
 
     def refresh(self):
         refresh_mx_weights([self])

@@ -940,3 +940,36 @@ def test_matmul_bits_dropped_with_an_8_bit_operand(p):
             assert bool((p.mx_matmul(a, b, out_dtype=torch.float32) == 2.0 ** e).all())
             got = p.mx_matmul(a, b)
             assert bool(((got.float() - 2.0 ** e).abs() <= 256 * 2.0 ** -13).all())
+
+
+# ---- what a caller may hand over, and what is refused ------------------------------------------------------------------------------------
+
+def test_weight_forms_handed_over_are_kept(p):
+    """A form that is handed over keeps its contents and its memory; what is missing is rounded from the parameter; a refresh renews both."""
+    g = torch.Generator().manual_seed(81)
+    w, other = (torch.randn(40, 72, generator=g) for _ in range(2))
+    param = torch.nn.Parameter(w.to(DEV))
+    for fmt in ("fp4", "fp8"):
+        own = [O.quantize(v, fmt) for v in (w, w.t())]
+        theirs = [O.quantize(v, fmt) for v in (other, other.t())]
+        for have_rows, have_cols, backward in ((True, False, True), (False, True, True), (True, True, True), (True, False, False), (False, True, False), (False, False, False)):
+            r, c = p.mx_quantize(other.to(DEV), fmt, which="both")
+            r, c = r if have_rows else None, c if have_cols else None
+            weight = p.MxWeight(param, fmt, backward=backward, rows=r, cols=c)
+            assert (r is None or weight.rows is r) and (c is None or weight.cols is c) and weight.fmt == fmt
+            _same(weight.rows, theirs[0] if have_rows else own[0], "rows")
+            assert (weight.cols is not None) == (have_cols or backward)
+            if weight.cols is not None:
+                _same(weight.cols, theirs[1] if have_cols else own[1], "cols")
+                x = torch.randn(3, 72, device=DEV, requires_grad=True)
+                (gx,) = torch.autograd.grad(p.mx_linear(x, weight).sum(), x)
+                assert gx.shape == x.shape
+            weight.refresh()
+            _same(weight.rows, own[0], "rows, refreshed")
+            if weight.cols is not None:
+                _same(weight.cols, own[1], "cols, refreshed")
+    r, c = p.mx_quantize(other.to(DEV), "fp8", which="both")
+    assert p.MxWeight(param, rows=r).fmt == p.MxWeight(param, cols=c).fmt == "fp8"               # the given form's, for both
+    _same(p.MxWeight(param, cols=c).rows, O.quantize(w, "fp8"), "rows")
+    with pytest.raises(p._lib.PsgdkError):
+        p.MxWeight(param, rows=r, cols=p.mx_quantize(other.to(DEV), "fp4", which="cols"))
