@@ -274,11 +274,11 @@ def _matmul(a, b, out_dtype, code):
 
 # ---------------------------------------------------------------------------------------------------------------------------- norm
 
-def _norm_args(x, gain, residual):
-    _tensor("x", x)
-    _dtype("x", x.dtype)
+def _norm_args(x, gain, residual, name="x", other="residual"):
+    _tensor(name, x)
+    _dtype(name, x.dtype)
     if x.dim() == 0 or x.shape[-1] == 0:
-        raise _bad(f"x of shape {tuple(x.shape)}: the norm needs at least one column")
+        raise _bad(f"{name} of shape {tuple(x.shape)}: the norm needs at least one column")
     if x.shape[-1] > NORM_MAX_COLS:
         raise L.PsgdkError(L.PSGDK_ERR_UNSUPPORTED, f"rms_norm_mx: {x.shape[-1]} columns, at most {NORM_MAX_COLS} (a row stays in registers)")
     _tensor("gain", gain, x.device)
@@ -286,9 +286,9 @@ def _norm_args(x, gain, residual):
     if gain.shape != x.shape[-1:]:
         raise _bad(f"gain of shape {tuple(gain.shape)} for rows of {x.shape[-1]}")
     if residual is not None:
-        _tensor("residual", residual, x.device)
+        _tensor(other, residual, x.device)
         if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise _bad(f"residual is {residual.dtype} {tuple(residual.shape)}, x is {x.dtype} {tuple(x.shape)}")
+            raise _bad(f"{other} is {residual.dtype} {tuple(residual.shape)}, {name} is {x.dtype} {tuple(x.shape)}")
 
 
 def rms_norm_mx(x: torch.Tensor, gain: torch.Tensor, residual: Optional[torch.Tensor] = None, *, eps: float = 1e-5, fmt: str = "fp8",
@@ -332,7 +332,7 @@ def rms_norm_mx_backward(dy: torch.Tensor, s: torch.Tensor, gain: torch.Tensor, 
     """(dx, dgain) of rms_norm_mx at the s and inv it returned, the rounding of y taken as the identity: with u = s inv,
     dx = inv (dy gain - u mean(dy gain u)) + ds -- the gradient of x and of the residual -- and dgain = the sum over rows of dy u (fp32, the same
     bits every run).  dy: s's dtype or fp32.  ds: the gradient that reaches s by its other uses."""
-    _norm_args(s, gain, ds)
+    _norm_args(s, gain, ds, "s", "ds")
     _tensor("dy", dy, s.device)
     _tensor("inv", inv, s.device)
     if dy.shape != s.shape or dy.dtype not in (s.dtype, torch.float32):

@@ -973,3 +973,14 @@ def test_weight_forms_handed_over_are_kept(p):
     _same(p.MxWeight(param, cols=c).rows, O.quantize(w, "fp8"), "rows")
     with pytest.raises(p._lib.PsgdkError):
         p.MxWeight(param, rows=r, cols=p.mx_quantize(other.to(DEV), "fp4", which="cols"))
+
+
+def test_norm_backward_names_what_it_refuses(p):
+    E = p._lib.PsgdkError
+    s, g, inv = torch.ones(4, 64, device=DEV), torch.ones(64, device=DEV), torch.ones(4, device=DEV)
+    for call, words in ((lambda: p.rms_norm_mx_backward(s, s, g, inv, ds=s[:3]), "ds is .*, s is "), (lambda: p.rms_norm_mx_backward(s, s, g, inv, ds=s.half()), "ds is .*, s is "),
+                        (lambda: p.rms_norm_mx_backward(s, s, g, inv, ds=s.cpu()), "ds lives on "), (lambda: p.rms_norm_mx_backward(s, s.cpu(), g, inv), "s lives on "),
+                        (lambda: p.rms_norm_mx_backward(s, s.double(), g, inv), "s has dtype "), (lambda: p.rms_norm_mx_backward(s, s[:, :0], g[:0], inv), "s of shape "),
+                        (lambda: p.rms_norm_mx(s, g, s[:3]), "residual is .*, x is ")):
+        with pytest.raises(E, match=words):
+            call()
