@@ -331,7 +331,8 @@ def _norm(x, gain, residual, eps, fmt, rows, cols):
 def rms_norm_mx_backward(dy: torch.Tensor, s: torch.Tensor, gain: torch.Tensor, inv: torch.Tensor, *, ds: Optional[torch.Tensor] = None):
     """(dx, dgain) of rms_norm_mx at the s and inv it returned, the rounding of y taken as the identity: with u = s inv,
     dx = inv (dy gain - u mean(dy gain u)) + ds -- the gradient of x and of the residual -- and dgain = the sum over rows of dy u (fp32, the same
-    bits every run).  dy: s's dtype or fp32.  ds: the gradient that reaches s by its other uses."""
+    bits every run).  dy: s's dtype or fp32.  ds: the gradient that reaches s by its other uses.  The results carry no gradient: in grad mode a dy, s, inv or ds
+    that requires one is refused; gain may be a parameter."""
     _norm_args(s, gain, ds, "s", "ds")
     _tensor("dy", dy, s.device)
     _tensor("inv", inv, s.device)
@@ -341,6 +342,8 @@ def rms_norm_mx_backward(dy: torch.Tensor, s: torch.Tensor, gain: torch.Tensor, 
     n = s.numel() // d
     if inv.dtype != torch.float32 or inv.numel() != n:
         raise _bad(f"inv: {n} values in float32, got {inv.dtype} {tuple(inv.shape)}")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (dy, s, inv, ds)):
+        raise _bad("rms_norm_mx_backward does not record gradients (there is no second backward pass): call it under torch.no_grad(), or on detached tensors")
     return _norm_backward(dy, s, gain, inv, ds)
 
 

@@ -984,3 +984,18 @@ def test_norm_backward_names_what_it_refuses(p):
                         (lambda: p.rms_norm_mx(s, g, s[:3]), "residual is .*, x is ")):
         with pytest.raises(E, match=words):
             call()
+
+
+def test_norm_backward_refuses_to_drop_gradients(p):
+    E = p._lib.PsgdkError
+    dy, s, ds = (torch.randn(4, 64, device=DEV) for _ in range(3))
+    inv, gain = torch.ones(4, device=DEV), torch.nn.Parameter(torch.ones(64, device=DEV))
+    want = p.rms_norm_mx_backward(dy, s, gain, inv, ds=ds)                        # a parameter as the gain is what a program has
+    assert not want[0].requires_grad and not want[1].requires_grad
+    for i in range(4):
+        a = [t.clone().requires_grad_(j == i) for j, t in enumerate((dy, s, inv, ds))]
+        with pytest.raises(E, match="does not record gradients"):
+            p.rms_norm_mx_backward(a[0], a[1], gain, a[2], ds=a[3])
+        with torch.no_grad():
+            got = p.rms_norm_mx_backward(a[0], a[1], gain, a[2], ds=a[3])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
