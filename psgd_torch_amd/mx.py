@@ -342,7 +342,7 @@ def rms_norm_mx_backward(dy: torch.Tensor, s: torch.Tensor, gain: torch.Tensor, 
     n = s.numel() // d
     if inv.dtype != torch.float32 or inv.numel() != n:
         raise _bad(f"inv: {n} values in float32, got {inv.dtype} {tuple(inv.shape)}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (dy, s, inv, ds)):
+    if torch.is_grad_enabled() and (dy.requires_grad or s.requires_grad or inv.requires_grad or ds is not None and ds.requires_grad):
         raise _bad("rms_norm_mx_backward does not record gradients (there is no second backward pass): call it under torch.no_grad(), or on detached tensors")
     return _norm_backward(dy, s, gain, inv, ds)
 
