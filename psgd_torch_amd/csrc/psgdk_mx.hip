@@ -75,6 +75,10 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
     if (t[f].rows == 0 || t[f].cols == 0) return PSGDK_OK;
     const bool rows = t[f].codes != nullptr, cols = t[f].codes_t != nullptr, noise = t[f].noise != nullptr;
     if ((!rows && !cols) || (noise && fmt != PSGDK_MX_FP4)) return PSGDK_ERR_INVALID;
+    const int64_t most = kMaxThreads / (cols ? 128 * mx_size(dtype) : 256);      // workgroups of a launch
+    // rows: units of 256 elements, 8 a workgroup; tiles: 128 x 128 over the padded extent of what is written
+    const auto across = [&](const psgdk_mx_tensor& q) { return cols ? (rows ? mx_pad(q.cols) : q.cols + 127) / 128 : mx_pad(q.cols) / MX_PAD; };
+    const auto needs = [&](const psgdk_mx_tensor& q) { return cols ? mx_pad(q.rows) / 128 * across(q) : (q.rows * across(q) + 7) / 8; };
     for (int i = 0; i < count; ++i) {
         const psgdk_mx_tensor& q = t[i];
         if (q.rows == 0 || q.cols == 0) continue;
@@ -82,8 +86,9 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
         if ((rows && !q.scales) || (cols && !q.scales_t)) return PSGDK_ERR_INVALID;
         if (!mx_aligned(q.x, mx_size(dtype)) || !mx_aligned(q.codes, 16) || !mx_aligned(q.codes_t, 16)) return PSGDK_ERR_INVALID;
     }
+    for (int i = 0; i < count; ++i)
+        if (t[i].rows && t[i].cols && needs(t[i]) > most) return PSGDK_ERR_UNSUPPORTED;          // (before the first launch: all of the tensors or none)
     const hipStream_t st = (hipStream_t)stream;
-    const int64_t most = kMaxThreads / (cols ? 128 * mx_size(dtype) : 256);      // workgroups of a launch
     for (int i = 0; i < count;) {
         MxJobs a;
         a.n = 0;
@@ -91,14 +96,11 @@ int psgdk_mx_quantize(int count, const psgdk_mx_tensor* t, int dtype, int fmt, v
         for (; i < count && a.n < MX_JOBS; ++i) {
             const psgdk_mx_tensor& q = t[i];
             if (q.rows == 0 || q.cols == 0) continue;
-            // rows: units of 256 elements, 8 a workgroup; tiles: 128 x 128 over the padded extent of what is written
-            const int64_t units = mx_pad(q.cols) / MX_PAD, tiles_n = (rows ? mx_pad(q.cols) : q.cols + 127) / 128;
-            const int64_t need = cols ? mx_pad(q.rows) / 128 * tiles_n : (q.rows * units + 7) / 8;
-            if (need > most) return PSGDK_ERR_UNSUPPORTED;
+            const int64_t need = needs(q);
             if (wgs + need > most) break;
             MxJob& j = a.j[a.n++];
             j = MxJob{q.x, (const uint8_t*)q.noise, (uint8_t*)q.codes, (uint8_t*)q.scales, (uint8_t*)q.codes_t, (uint8_t*)q.scales_t, q.ld, (int)q.rows,
-                      (int)q.cols, (unsigned)wgs, FastDiv::make((unsigned)(cols ? tiles_n : units))};
+                      (int)q.cols, (unsigned)wgs, FastDiv::make((unsigned)across(q))};
             wgs += need;
         }
         if (a.n == 0) continue;

@@ -254,3 +254,11 @@ def test_plan_query(lib):
     for bad in ((0, 1, 1, 4, 4, 0), (1, 0, 1, 4, 4, 0), (1, 1, -1, 4, 4, 0), (1, 1, 1, 5, 4, 0), (1, 1, 1, 4, 5, 0), (1, 1, 1, 4, 4, 3), (1 << 31, 1, 1, 4, 4, 0)):
         assert plan(*bad)[0] == 1
     assert lib.psgdk_test_mx_plan(1, 1, 1, 4, 4, 0, None, None, None, None) == 1
+
+
+def test_quantize_refuses_before_it_launches(lib):
+    """One tensor too large for a launch behind 32 others, which fill a launch of their own: refused as a whole."""
+    from psgd_torch_amd import _lib
+    for kw in (dict(), dict(codes=None, scales=None, codes_t=8192, scales_t=8192)):
+        ts = (_lib.MxTensorArg * 33)(*[_arg(**kw) for _ in range(32)], _arg(rows=1 << 30, cols=1024, ld=1 << 10, **kw))
+        assert lib.psgdk_mx_quantize(33, ts, 1, 4, None) == 2
