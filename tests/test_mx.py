@@ -262,3 +262,19 @@ def test_quantize_refuses_before_it_launches(lib):
     for kw in (dict(), dict(codes=None, scales=None, codes_t=8192, scales_t=8192)):
         ts = (_lib.MxTensorArg * 33)(*[_arg(**kw) for _ in range(32)], _arg(rows=1 << 30, cols=1024, ld=1 << 10, **kw))
         assert lib.psgdk_mx_quantize(33, ts, 1, 4, None) == 2
+
+
+def test_negated_views_are_resolved():
+    """The imaginary part of a conjugated tensor has memory of the other sign, contiguous where it has one column or one element: kernels read memory."""
+    from psgd_torch_amd import mx
+
+    def memory(t):
+        return [C.c_float.from_address(t.data_ptr() + 4 * i * t.stride(0)).value for i in range(t.shape[0])]
+    z = torch.complex(torch.zeros(5, 1), torch.arange(1.0, 6.0)[:, None]).conj()
+    x = z.imag
+    assert x.is_neg() and x[:, 0].tolist() == [-1.0, -2.0, -3.0, -4.0, -5.0] and memory(x) == [1.0, 2.0, 3.0, 4.0, 5.0]
+    assert memory(mx._rows("x", x)) == memory(mx._flat(x)) == x[:, 0].tolist()
+    one = z[:1].imag
+    assert one.is_neg() and one.is_contiguous() and memory(mx._flat(one)) == [-1.0]
+    plain = torch.ones(3, 4)
+    assert mx._flat(plain) is plain and mx._rows("x", plain) is plain
