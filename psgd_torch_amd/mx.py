@@ -70,12 +70,12 @@ def _rows(what, x) -> torch.Tensor:
         x = x.reshape(n, x.shape[-1])
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         x = x.contiguous()
-    return x.resolve_neg() if x.is_neg() else x
+    return _flat(x) if x.shape[1] == 1 else x
 
 
 def _flat(t) -> torch.Tensor:
-    """t with contiguous elements that are what they read as (the imaginary part of a conjugated tensor is a view whose memory has the other sign)."""
-    t = t.contiguous()
+    """t with memory that is what it reads as.  The imaginary part of a conjugated tensor is a view of memory with the other sign and with gaps, which
+    contiguous() resolves; where one element a row or one at all is left there are no gaps, and it does not."""
     return t.resolve_neg() if t.is_neg() else t
 
 
@@ -318,13 +318,17 @@ def rms_norm_mx(x: torch.Tensor, gain: torch.Tensor, residual: Optional[torch.Te
 def _norm(x, gain, residual, eps, fmt, rows, cols):
     """(y or None, y transposed or None, s, inv) of checked arguments."""
     d = x.shape[-1]
-    x, gain = _flat(x), _flat(gain)
+    x, gain = x.contiguous(), gain.contiguous()
+    if d == 1:
+        x, gain = _flat(x), _flat(gain)
     n = x.numel() // d
     device = x.device
     if residual is None:
         s, res = x, None
     else:
-        residual = _flat(residual)
+        residual = residual.contiguous()
+        if d == 1:
+            residual = _flat(residual)
         s, res = torch.empty_like(x), residual.data_ptr()
     inv = torch.empty(n, dtype=torch.float32, device=device)
     r = MxTensor.empty(n, d, fmt, device) if rows else None
@@ -354,11 +358,13 @@ def rms_norm_mx_backward(dy: torch.Tensor, s: torch.Tensor, gain: torch.Tensor, 
 
 
 def _norm_backward(dy, s, gain, inv, ds):
-    dy, s, gain, inv = _flat(dy), _flat(s), _flat(gain), _flat(inv)
+    dy, s, gain, inv = dy.contiguous(), s.contiguous(), gain.contiguous(), inv.contiguous()
     if ds is not None:
-        ds = _flat(ds)
+        ds = ds.contiguous()
     d = s.shape[-1]
     n = s.numel() // d
+    if d == 1 or n == 1:
+        dy, s, gain, inv, ds = _flat(dy), _flat(s), _flat(gain), _flat(inv), None if ds is None else _flat(ds)
     device = s.device
     dx = torch.empty_like(s)
     dgain = torch.empty(d, dtype=torch.float32, device=device)

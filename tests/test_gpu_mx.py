@@ -999,3 +999,19 @@ def test_norm_backward_refuses_to_drop_gradients(p):
         with torch.no_grad():
             got = p.rms_norm_mx_backward(a[0], a[1], gain, a[2], ds=a[3])
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("shape", [(5, 1), (1, 1), (3, 7), (1, 40)])
+def test_negated_views(p, shape):
+    """Imaginary parts of conjugated tensors: views whose memory has the other sign."""
+    g = torch.Generator().manual_seed(82)
+    x, r, gain = (torch.randn(s, generator=g).to(DEV) for s in (shape, shape, shape[1:]))
+    neg = lambda t: torch.complex(torch.zeros_like(t), -t).conj().imag      # noqa: E731  (reads as t)
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    a, b = p.mx_quantize(neg(x), which="both"), p.mx_quantize(x, which="both")
+    assert all(torch.equal(i.codes, j.codes) and torch.equal(i.scales, j.scales) for i, j in zip(a, b))
+    ya, sa, ia = p.rms_norm_mx(neg(x), neg(gain), neg(r))
+    yb, sb, ib = p.rms_norm_mx(x, gain, r)
+    assert torch.equal(ya.codes, yb.codes) and torch.equal(sa, sb) and torch.equal(ia, ib)
+    da, db = p.rms_norm_mx_backward(neg(x), neg(sb), neg(gain), neg(ib), ds=neg(r)), p.rms_norm_mx_backward(x, sb, gain, ib, ds=r)
+    assert torch.equal(da[0], db[0]) and torch.equal(da[1], db[1])
