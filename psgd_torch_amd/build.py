@@ -36,6 +36,12 @@ def needs_build() -> bool:
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
+def object_command(hipcc, src, obj):
+    """Compiles one unit.  Its id is its name: hipcc would make one of the whole command line, so that objects of the same source in another temporary
+    folder, and with them the library, would differ from build to build (profiles carry the hash of the library that they measured)."""
+    return [hipcc, *FLAGS, "-cuid=" + os.path.splitext(os.path.basename(src))[0], "-c", src, "-o", obj]
+
+
 def _run(cmds, verbose):
     """Runs the commands side by side; the first that fails raises with its output."""
     procs = []
@@ -55,7 +61,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     with tempfile.TemporaryDirectory() as tmp:
         objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in SRCS]
-        _run([[hipcc, *FLAGS, "-c", s, "-o", o] for s, o in zip(SRCS, objs)]
+        _run([object_command(hipcc, s, o) for s, o in zip(SRCS, objs)]
              + [[hipcc, *FLAGS, "-shared", PROBE_SRC, "-o", PROBE_OUT]], verbose)
         _run([[hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", OUT]], verbose)
     return OUT
