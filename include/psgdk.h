@@ -412,7 +412,8 @@ int psgdk_mx_matmul_work_bytes(int64_t m, int64_t n, int64_t k, int a_fmt, int b
 int psgdk_mx_matmul(const void* a_codes, const void* a_scales, int64_t m, int a_fmt, const void* b_codes, const void* b_scales, int64_t n, int b_fmt,
                     int64_t k, void* out, int out_dtype, void* work, size_t work_bytes, void* stream);
 /* s = x + residual, rounded to dtype (residual NULL: s is x, nothing is written); inv = (mean of s^2 + eps)^-1/2 of every row, squares and sum in
- * 64 bits, rounded once; y = s inv gain, rounded once from fp32, in MX form (codes), and y transposed in MX form (codes_t); either may be NULL.  cols <= PSGDK_NORM_MAX_COLS.  s may be x or residual. */
+ * 64 bits, rounded once; y = s inv gain, rounded once from fp32, in MX form (codes), and y transposed in MX form (codes_t); either may be NULL.
+ * cols <= PSGDK_NORM_MAX_COLS.  s may be x or residual. */
 int psgdk_rms_norm_mx(const void* x, const void* residual, const void* gain, int gain_dtype, int64_t rows, int64_t cols, int dtype, float eps, int fmt,
                       void* s, float* inv, void* codes, void* scales, void* codes_t, void* scales_t, void* stream);
 /* dx = inv (dy gain - u mean(dy gain u)) + ds with u = s inv (the gradient of x and of the residual; ds, the gradient that reaches s by its other

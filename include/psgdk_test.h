@@ -94,8 +94,9 @@ int psgdk_test_trsm_bench(const void* Y, const void* U, const void* Ut, void* ou
 int psgdk_test_tile_queues(int n, const int32_t* M, const int32_t* N, const int32_t* K, const int32_t* sym, int big,
                            int64_t* queue_tiles, int64_t* queue_cost, int64_t* table_len);
 
-/* Host-only: what psgdk_mx_matmul chooses for a product.  rows x cols: its tile (cols = 0: the few-rows kernel, rows = the rows of A it holds); splits: the parts K
- * is cut in (the few-rows kernel: waves that share a group of rows of B); wide: 1 where 8-bit elements are multiplied as bf16. */
+/* Host-only: what psgdk_mx_matmul chooses for a product.  rows x cols: its tile (cols = 0: the few-rows kernel, rows = the rows of A
+ * it holds); splits: the parts K is cut in (the few-rows kernel: waves that share a group of rows of B); wide: 1 where 8-bit elements
+ * are multiplied as bf16. */
 int psgdk_test_mx_plan(int64_t m, int64_t n, int64_t k, int a_fmt, int b_fmt, int out_dtype, int* rows, int* cols, int* splits, int* wide);
 
 #ifdef __cplusplus
